@@ -9,9 +9,16 @@ void Booster::set_param(const std::string& key, const std::string& value) {
   params_changed_ = true;
 }
 
-void Booster::update_one_iter(int iter, DMatrix* d) {
+void Booster::update_one_iter(int iter, DMatrix* d, const CallerGradients* caller) {
   need(d != nullptr, "training matrix handle is null");
   need(iter >= 0, "iteration must be non-negative");
+  bind(d, caller == nullptr);
+  engine_->profiler().enable(profiling);
+  engine_->boost_round(model, caller);
+  ++model_version_;
+}
+
+Engine& Booster::bind(DMatrix* d, bool need_labels) {
   const int K = params.K();
   need(K >= 1, "num_class must be at least 1 for multi-class objectives");
   if (params.objective.rfind("multi:", 0) == 0) need(params.num_class >= 2, "num_class must be at least 2");
@@ -23,7 +30,7 @@ void Booster::update_one_iter(int iter, DMatrix* d) {
     need(model.trees.empty(),
          "continuing training on a different matrix, objective, num_class or max_bin is not supported");
     engine_.reset();
-    engine_ = std::make_unique<Engine>(*d, params, comm);
+    engine_ = std::make_unique<Engine>(*d, params, comm, need_labels);
     engine_objective_ = params.objective;
     engine_classes_ = K;
     engine_max_bin_ = params.max_bin;
@@ -32,9 +39,7 @@ void Booster::update_one_iter(int iter, DMatrix* d) {
     engine_->update_params(params);
   }
   params_changed_ = false;
-  engine_->profiler().enable(profiling);
-  engine_->boost_round(model);
-  ++model_version_;
+  return *engine_;
 }
 
 const std::string& Booster::save_model_json() {

@@ -23,7 +23,11 @@ class Booster {
   int profiling = 0;  // profiler mode (see Profiler::enable)
 
   void set_param(const std::string& key, const std::string& value);
-  void update_one_iter(int iter, DMatrix* d);
+  // One round on the objective's gradients, or on a caller's (then the matrix
+  // needs no labels).
+  void update_one_iter(int iter, DMatrix* d, const CallerGradients* caller = nullptr);
+  // The engine bound to a training matrix, made or updated as the parameters ask.
+  Engine& bind(DMatrix* d, bool need_labels);
   int boosted_rounds() const { return model.rounds(); }
   const std::string& save_model_json();
   const std::string& save_config_json();

@@ -270,6 +270,62 @@ int XGBoosterUpdateOneIter(BoosterHandle handle, int iter, DMatrixHandle dtrain)
   DP_API_END();
 }
 
+namespace {
+// A caller's gradients or curvatures of a round: fp32 device memory, [rows]
+// (one output) or [rows, outputs], outputs adjacent.
+const float* round_array(const char* text, const char* what, const dp::DMatrix& d, dp::u64 outputs, dp::u64* stride) {
+  const std::string w(what);
+  const ArrayInterface a = parse_array(text);
+  need(a.typestr == "<f4", w + " must be little-endian float32 (<f4)");
+  need((a.shape.size() == 2 && a.shape[1] == outputs) || (a.shape.size() == 1 && outputs == 1),
+       w + " must have the shape [rows, outputs] (one output: also [rows])");
+  need(a.shape[0] == d.rows(), w + " must have one row for every row of the training matrix");
+  *stride = outputs;
+  if (!a.strides.empty()) {
+    need(a.strides.size() == a.shape.size(), w + " strides must match its shape");
+    need(outputs == 1 || a.strides[1] == 4, w + " must hold a row's outputs next to each other");
+    need(a.shape[0] <= 1 || (a.strides[0] % 4 == 0 && a.strides[0] / 4 >= dp::i64(outputs) &&
+                             a.strides[0] / 4 <= (dp::i64(1) << 31)),
+         w + " row stride must cover the outputs");
+    if (a.shape[0] > 1) *stride = dp::u64(a.strides[0]) / 4;
+  }
+  need(a.shape[0] == 0 || a.ptr != 0, w + " pointer is null");
+  need(a.ptr % 4 == 0, w + " pointer is not aligned to 4 bytes");
+  const float* p = reinterpret_cast<const float*>(a.ptr);
+  if (a.shape[0]) need(pointer_device(p, false) == d.device(), w + " must be on the training matrix's device");
+  return p;
+}
+}  // namespace
+
+int XGBoosterTrainOneIter(BoosterHandle handle, DMatrixHandle dtrain, int iter, const char* grad, const char* hess) {
+  DP_API_BEGIN();
+  dp::Booster* b = as_booster(handle);
+  dp::DMatrix* d = as_dmatrix(dtrain);
+  need(b->params.K() >= 1, "num_class must be at least 1 for multi-class objectives");
+  dp::CallerGradients c;
+  c.grad = round_array(grad, "grad", *d, dp::u64(b->params.K()), &c.grad_stride);
+  c.hess = round_array(hess, "hess", *d, dp::u64(b->params.K()), &c.hess_stride);
+  {
+    dp::DeviceGuard g(d->device());
+    // the producer may still be writing on its own stream
+    dp::cuda_check(cudaDeviceSynchronize(), "synchronise producer");
+  }
+  b->update_one_iter(iter, d, &c);
+  DP_API_END();
+}
+
+int dp_booster_train_margin(BoosterHandle handle, DMatrixHandle dtrain, bst_ulong* out_rows, bst_ulong* out_outputs,
+                            const float** out) {
+  DP_API_BEGIN();
+  need(out_rows != nullptr && out_outputs != nullptr && out != nullptr, "output pointer is null");
+  dp::Booster* b = as_booster(handle);
+  dp::DMatrix* d = as_dmatrix(dtrain);
+  *out = b->bind(d, false).device_margins();
+  *out_rows = d->rows();
+  *out_outputs = bst_ulong(b->params.K());
+  DP_API_END();
+}
+
 int XGBoosterBoostedRounds(BoosterHandle handle, int* out) {
   DP_API_BEGIN();
   need(out != nullptr, "output pointer is null");

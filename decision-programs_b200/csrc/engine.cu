@@ -140,10 +140,11 @@ u64 env_u64(const char* name, u64 dflt) {
 }
 }
 
-Engine::Engine(DMatrix& d, const TrainParams& p, Comm* comm) : d_(d), p_(p), comm_(comm), device_(d.device()) {
+Engine::Engine(DMatrix& d, const TrainParams& p, Comm* comm, bool need_labels)
+    : d_(d), p_(p), comm_(comm), device_(d.device()) {
   DeviceGuard g(device_);
   DP_CUDA(cudaStreamCreateWithFlags(&stream_, cudaStreamNonBlocking));
-  need(d_.has_labels(), "training matrix has no labels");
+  need(!need_labels || d_.has_labels(), "training matrix has no labels");
   K_ = p_.K();
   need(K_ >= 1, "num_class must be set for multi-class objectives");
   R_ = d_.rows();
@@ -243,10 +244,8 @@ Engine::Engine(DMatrix& d, const TrainParams& p, Comm* comm) : d_(d), p_(p), com
   std::vector<float> base(K_);
   for (int k = 0; k < K_; ++k) base[k] = p_.base_margin(k);
   float* base_d = reinterpret_cast<float*>(scratch_.get() + 1);
-  DP_CUDA(cudaMemsetAsync(scratch_.get(), 0, sizeof(u32), stream_));
   // the last-block counters start at zero (a reused slab holds old data)
   DP_CUDA(cudaMemsetAsync(done_.get(), 0, done_.size() * sizeof(u32), stream_));
-  launch_check_labels(d_.labels(), R_, p_.objective_id(), K_, scratch_.get(), stream_);
   std::memcpy(arena_.get() + kArenaHead, base.data(), K_ * sizeof(float));
   DP_CUDA(cudaMemcpyAsync(base_d, arena_.get() + kArenaHead, K_ * sizeof(float), cudaMemcpyHostToDevice, stream_));
   launch_init_margins(margin_.get(), std::max<u64>(R_, 1), K_, base_d, stream_);
@@ -255,6 +254,15 @@ Engine::Engine(DMatrix& d, const TrainParams& p, Comm* comm) : d_(d), p_(p), com
     for (int k = 0; k < K_; ++k) ta[s * K_ + k] = TreeArrays{ridx_[s].get() + u64(k) * R_, gh_[s].get() + u64(k) * R_};
   DP_CUDA(cudaMemcpy(tarr_[0].get(), ta.data(), K_ * sizeof(TreeArrays), cudaMemcpyHostToDevice));
   DP_CUDA(cudaMemcpy(tarr_[1].get(), ta.data() + K_, K_ * sizeof(TreeArrays), cudaMemcpyHostToDevice));
+  if (need_labels) check_labels();
+  else sync_stream();
+  prof_.host("engine_init", ms_since(t0));
+}
+
+void Engine::check_labels() {
+  need(d_.has_labels(), "training matrix has no labels");
+  DP_CUDA(cudaMemsetAsync(scratch_.get(), 0, sizeof(u32), stream_));
+  launch_check_labels(d_.labels(), R_, p_.objective_id(), K_, scratch_.get(), stream_);
   u32 bad = 0;
   DP_CUDA(cudaMemcpyAsync(&bad, scratch_.get(), sizeof(u32), cudaMemcpyDeviceToHost, stream_));
   sync_stream();
@@ -264,7 +272,7 @@ Engine::Engine(DMatrix& d, const TrainParams& p, Comm* comm) : d_(d), p_(p), com
       fail("label must be an integer in [0, num_class) for multi-class objectives");
     fail("label contains NaN or infinity");
   }
-  prof_.host("engine_init", ms_since(t0));
+  labels_checked_ = true;
 }
 
 Engine::~Engine() {
@@ -469,8 +477,30 @@ void Engine::drop_graph() {
   prof_.drop_graph();
 }
 
-void Engine::boost_round(Model& m) {
+RowSample Engine::row_sample() const {
+  RowSample rs;
+  if (row_sampling()) rs = RowSample{p_.subsample, p_.seed, round_dev_.get(), row0_};
+  return rs;
+}
+
+// A caller's gradients of this round into (g, h) pairs, before the launches a
+// graph may hold (their addresses change from round to round).  All ranks
+// refuse the round when one of them finds a value that cannot be quantised.
+void Engine::load_gradients(const CallerGradients& c) {
+  u32* const gmax = ghmax_.get();
+  DP_CUDA(cudaMemsetAsync(scratch_.get(), 0, sizeof(u32), stream_));
+  DP_CUDA(cudaMemsetAsync(gmax, 0, 2 * size_t(K_) * sizeof(u32), stream_));
+  launch_caller_gradients(c, K_, R_, gh_[0].get(), gmax, gmax + K_, scratch_.get(), stream_, row_sample());
+  if (comm_ && G_ > 1) comm_->max_u32(scratch_.get(), 1, stream_);
+  u32* const bad = reinterpret_cast<u32*>(arena_.get() + 192);  // in the arena's head
+  DP_CUDA(cudaMemcpyAsync(bad, scratch_.get(), sizeof(u32), cudaMemcpyDeviceToHost, stream_));
+  sync_stream();
+  if (*bad) fail("gradients must be finite, and curvatures finite and not negative");
+}
+
+void Engine::boost_round(Model& m, const CallerGradients* caller) {
   DeviceGuard g(device_);
+  if (!caller && !labels_checked_) check_labels();
   NvtxRange nv("dp_gbdt: boosting round");
   const auto t_round = std::chrono::steady_clock::now();
   // Rounds after the first replay one CUDA graph of the whole round when every
@@ -485,8 +515,9 @@ void Engine::boost_round(Model& m) {
     *r_h = u32(m.rounds());
     DP_CUDA(cudaMemcpyAsync(round_dev_.get(), r_h, sizeof(u32), cudaMemcpyHostToDevice, stream_));
   }
+  if (caller) load_gradients(*caller);
   RoundOut out;
-  if (graphable && graph_exec_ && graph_prof_ == prof_.mode()) {
+  if (graphable && graph_exec_ && graph_prof_ == prof_.mode() && graph_caller_ == (caller != nullptr)) {
     DP_CUDA(cudaGraphLaunch(graph_exec_, stream_));
     count_launch(graph_launches_);
     prof_.graph_round();
@@ -499,7 +530,7 @@ void Engine::boost_round(Model& m) {
     bool captured = false;
     DP_CUDA(cudaStreamBeginCapture(stream_, cudaStreamCaptureModeThreadLocal));
     try {
-      out = enqueue_round();
+      out = enqueue_round(caller != nullptr);
       captured = cudaStreamEndCapture(stream_, &graph_) == cudaSuccess && graph_ != nullptr;
     } catch (...) {
       cudaGraph_t partial = nullptr;
@@ -513,6 +544,7 @@ void Engine::boost_round(Model& m) {
       prof_.finish_capture();
       graph_launches_ = n;
       graph_prof_ = prof_.mode();
+      graph_caller_ = caller != nullptr;
       graph_out_ = out;
       DP_CUDA(cudaGraphLaunch(graph_exec_, stream_));
       count_launch(graph_launches_);
@@ -523,10 +555,10 @@ void Engine::boost_round(Model& m) {
       prof_.abort_capture();
       drop_graph();
       graphs_ = false;
-      out = enqueue_round();
+      out = enqueue_round(caller != nullptr);
     }
   } else {
-    out = enqueue_round();
+    out = enqueue_round(caller != nullptr);
   }
   prof_.host("round_enqueue", ms_since(t_round));
   finish_round(m, out);
@@ -534,7 +566,7 @@ void Engine::boost_round(Model& m) {
   ++rounds_;
 }
 
-Engine::RoundOut Engine::enqueue_round() {
+Engine::RoundOut Engine::enqueue_round(bool caller) {
   const int K = K_;
   const u64 R = R_;
   const u32 F = F_;
@@ -562,18 +594,19 @@ Engine::RoundOut Engine::enqueue_round() {
   // ---- gradients and quantiser scales.  Up to 64 classes the maxima are
   // reduced by the gradient launch's last block (with one rank it also
   // computes the scales); beyond, per-class atomics on zeroed maxima.
-  prof_.begin(stream_, "gradients", double(R) * K * (4 + 8) + double(R) * 4);
-  RowSample rs;
-  if (row_sampling()) rs = RowSample{p_.subsample, p_.seed, round_dev_.get(), row0_};
-  const bool reduced = K <= kMaxReducedClasses;
-  if (reduced) {
+  const RowSample rs = row_sample();
+  const bool reduced = K <= kMaxReducedClasses && !caller;
+  if (!caller) prof_.begin(stream_, "gradients", double(R) * K * (4 + 8) + double(R) * 4);
+  if (caller) {
+    // load_gradients has written the pairs and their maxima
+  } else if (reduced) {
     launch_gradients_reduced(p_.objective_id(), K, margin_.get(), d_.labels(), R, gh_[0].get(), gmax, hmax,
                              max_part_.get(), done_.get(), one_rank ? scales_.get() : nullptr, stream_, rs);
   } else {
     DP_CUDA(cudaMemsetAsync(gmax, 0, 2 * size_t(K) * sizeof(u32), stream_));
     launch_gradients(p_.objective_id(), K, margin_.get(), d_.labels(), R, gh_[0].get(), gmax, hmax, stream_, rs);
   }
-  prof_.end(stream_);
+  if (!caller) prof_.end(stream_);
   if (!one_rank) comm_->max_u32(gmax, 2 * size_t(K), stream_);
   if (!reduced || !one_rank) launch_scales(K, gmax, hmax, scales_.get(), stream_);
   // (g, h) become exact int32 pairs once per round (every later pass reads

@@ -79,12 +79,16 @@ class Profiler {
 
 class Engine {
  public:
-  Engine(DMatrix& d, const TrainParams& p, Comm* comm);
+  // need_labels: the objective's own gradients will be used (they read the
+  // labels, which are checked here); without, boost_round checks them when it
+  // is first called without a caller's gradients.
+  Engine(DMatrix& d, const TrainParams& p, Comm* comm, bool need_labels = true);
   ~Engine();
   Engine(const Engine&) = delete;
   Engine& operator=(const Engine&) = delete;
 
-  void boost_round(Model& m);
+  // One round on the objective's gradients, or on a caller's.
+  void boost_round(Model& m, const CallerGradients* caller = nullptr);
   // Regularisation / depth / learning-rate changes between rounds.
   void update_params(const TrainParams& p) {
     p_ = p;
@@ -95,6 +99,8 @@ class Engine {
   cudaStream_t stream() const { return stream_; }
   // Training margins [R][K] copied to host.
   std::vector<float> margins() const;
+  // The same on the device; complete between rounds.
+  const float* device_margins() const { return margin_.get(); }
 
  private:
   void sync();
@@ -129,7 +135,12 @@ class Engine {
     u64 ids_hi = 1;                             // bound on node ids per tree
     std::vector<int> pi_hist, pi_eval;          // profiler entries per level
   };
-  RoundOut enqueue_round();                       // every launch of one round
+  // Every launch of one round; with a caller's gradients those that follow
+  // load_gradients.
+  RoundOut enqueue_round(bool caller);
+  void load_gradients(const CallerGradients& c);
+  void check_labels();
+  RowSample row_sample() const;
   void finish_round(Model& m, const RoundOut& out);  // one read-back, the trees
   bool all_levels_async() const;
   bool row_sampling() const { return p_.subsample < 1.0; }
@@ -212,6 +223,8 @@ class Engine {
   u64 dev_round_ = ~u64(0);  // value of round_dev_ when known
   int sms_ = 148;
   // CUDA graph of a whole round (replayed while the bounds and buffers hold)
+  bool labels_checked_ = false;
+  bool graph_caller_ = false;  // the graph starts after a caller's gradients
   bool graphs_ = true;  // DP_CUDA_GRAPHS=0 turns capture off
   // The last level adds leaf values while routing rows instead of moving
   // them (DP_FOLD_LAST_LEVEL=0: moves them and updates margins afterwards).

@@ -128,6 +128,46 @@ __global__ void __launch_bounds__(256) k_gradients(int objective, int K, const f
   }
 }
 
+// One thread a row, walking its classes: writes are coalesced (class-major),
+// and a row's reads share their lines in L1.  Memory-bound: 16 B per (row,
+// class); maxima go through shared counters for up to kSharedClasses classes.
+__global__ void __launch_bounds__(256) k_caller_gradients(CallerGradients c, int K, u64 R, float2* __restrict__ gh,
+                                                           u32* gmax, u32* hmax, u32* bad, RowSample rs) {
+  __shared__ u32 smg[kSharedClasses], smh[kSharedClasses];
+  const bool sampling = rs.rate < 1.0, shared_max = K <= kSharedClasses;
+  const u32 round = sampling ? *rs.round : 0u;
+  for (int k = threadIdx.x; k < kSharedClasses; k += blockDim.x) { smg[k] = 0u; smh[k] = 0u; }
+  __syncthreads();
+  bool wrong = false;
+  const u64 step = u64(gridDim.x) * blockDim.x;
+  for (u64 base = u64(blockIdx.x) * blockDim.x; base < R; base += step) {
+    const u64 r = base + threadIdx.x;
+    for (int k = 0; k < K; ++k) {
+      float g = 0.f, h = 0.f;
+      if (r < R) {
+        g = c.grad[r * c.grad_stride + u64(k)];
+        h = c.hess[r * c.hess_stride + u64(k)];
+        wrong |= !isfinite(g) || !(h >= 0.f) || isinf(h);
+        if (sampling && !(sample_uniform(sample_hash(rs.seed, round, u32(k), kSampleRow, rs.row0 + r, 0)) < rs.rate))
+          g = h = 0.f;
+        gh[u64(k) * R + r] = make_float2(g, h);
+      }
+      const u32 wg = warp_max(__float_as_uint(fabsf(g))), wh = warp_max(__float_as_uint(fabsf(h)));
+      if ((threadIdx.x & 31) == 0 && (wg | wh)) {
+        atomicMax((shared_max ? smg : gmax) + k, wg);
+        atomicMax((shared_max ? smh : hmax) + k, wh);
+      }
+    }
+  }
+  if (__any_sync(0xffffffffu, wrong) && (threadIdx.x & 31) == 0) atomicOr(bad, 1u);
+  __syncthreads();
+  if (shared_max)
+    for (int k = threadIdx.x; k < K; k += blockDim.x) {
+      if (smg[k]) atomicMax(gmax + k, smg[k]);
+      if (smh[k]) atomicMax(hmax + k, smh[k]);
+    }
+}
+
 __global__ void __launch_bounds__(256) k_quantize_gh(float2* gh, u64 R, int K, const Scales* __restrict__ sc) {
   const u64 n = R * u64(K);
   for (u64 i = u64(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += u64(gridDim.x) * blockDim.x) {
@@ -254,6 +294,14 @@ void launch_gradients_reduced(int objective, int K, const float* margin, const f
   k_gradients<<<grid_for(R, 256), 256, 0, s>>>(objective, K, margin, label, R, gh, gmax_bits, hmax_bits, rs, part,
                                                 done, scales);
   after_launch("gradients");
+}
+
+void launch_caller_gradients(const CallerGradients& c, int K, u64 R, float2* gh, u32* gmax_bits, u32* hmax_bits,
+                             u32* bad, cudaStream_t s, const RowSample& rs) {
+  if (R == 0) return;
+  need(rs.rate >= 1.0 || rs.round != nullptr, "row sampling needs the round counter");
+  k_caller_gradients<<<grid_for(R, 256), 256, 0, s>>>(c, K, R, gh, gmax_bits, hmax_bits, bad, rs);
+  after_launch("caller gradients");
 }
 
 void launch_scales(int K, const u32* gmax_bits, const u32* hmax_bits, Scales* scales, cudaStream_t s) {

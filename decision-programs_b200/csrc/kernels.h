@@ -140,6 +140,18 @@ void launch_scales(int K, const u32* gmax_bits, const u32* hmax_bits, Scales* sc
 // scales (launch_scales' formula).  *done must be zero at the first launch;
 // every launch leaves it zero.  Launches one block even for R == 0.
 constexpr int kMaxReducedClasses = 64;
+// A caller's gradients and curvatures ([rows][K] fp32, device, rows
+// grad_stride / hess_stride elements apart) of one round.
+struct CallerGradients {
+  const float* grad = nullptr;
+  const float* hess = nullptr;
+  u64 grad_stride = 0, hess_stride = 0;
+};
+// gh[K][R] (g, h) pairs from a caller's gradients, with the row sampling of
+// the round and the maxima of |g| and h (gmax / hmax zeroed before); sets *bad
+// when a gradient is not finite or a curvature not finite or negative.
+void launch_caller_gradients(const CallerGradients& c, int K, u64 R, float2* gh, u32* gmax_bits, u32* hmax_bits,
+                             u32* bad, cudaStream_t s, const RowSample& rs);
 u32 gradient_blocks(u64 R);
 void launch_gradients_reduced(int objective, int K, const float* margin, const float* label, u64 R, float2* gh,
                               u32* gmax_bits, u32* hmax_bits, u32* part, u32* done, Scales* scales, cudaStream_t s,

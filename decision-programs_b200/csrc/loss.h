@@ -1,0 +1,76 @@
+// Losses that learn from choices: log-probabilities of a chosen class and
+// their backward pass, the clipped policy loss, and the preference loss over
+// pairs (dp_log_prob, dp_log_prob_grad, dp_policy_loss, dp_preference_* in
+// include/dp_gbdt.h).  Launchers take device pointers, enqueue on `s` and
+// never synchronise or allocate.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "common.h"
+
+namespace dp {
+
+enum MarginType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+inline u64 margin_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+// Margins [rows][classes], rows `stride` elements apart.
+struct Margins {
+  const void* z = nullptr;
+  int dtype = kF32;
+  u64 rows = 0;
+  u32 classes = 0;
+  u64 stride = 0;
+};
+// Gradient in the margins' type and curvature in fp32; null when not wanted.
+struct MarginGrad {
+  void* grad = nullptr;
+  u64 grad_stride = 0;
+  float* hess = nullptr;
+  u64 hess_stride = 0;
+};
+struct PolicyRows {
+  const float* old_log_prob = nullptr;
+  const float* ref_log_prob = nullptr;  // null: no KL term
+  const float* advantage = nullptr;
+  const float* weight = nullptr;  // null: 1
+  float clip_low = 0.f, clip_high = 0.f, kl = 0.f;
+};
+
+void launch_log_prob(const Margins& m, const i32* label, float* log_prob, float2* norm, cudaStream_t s);
+void launch_log_prob_grad(const Margins& m, const i32* label, const float2* norm, const float* weight,
+                          const MarginGrad& out, cudaStream_t s);
+void launch_policy_loss(const Margins& m, const i32* label, const PolicyRows& p, float* loss, float* log_prob,
+                        const MarginGrad& out, cudaStream_t s);
+
+// Scores of items: item i is rows [begin[i], begin[i + 1]) of score (begin
+// null: row i); pair p is items 2p (preferred) and 2p + 1.
+struct PairLoss {
+  const float* score = nullptr;
+  const float* ref = nullptr;     // null: no reference model
+  const float* weight = nullptr;  // per pair; null: 1
+  float beta = 1.f, smoothing = 0.f;
+  float* loss = nullptr;  // [pairs]
+  float* grad = nullptr;  // [rows]
+  float* hess = nullptr;  // [rows] or null
+};
+void launch_preference(const PairLoss& a, u64 rows, const i64* begin, u64 pairs, cudaStream_t s);
+
+// Any pairs over rows, laid out by row once: the pairs that row r takes part
+// in are entries [off[r], off[r + 1]) in ascending order of the pair.
+struct PairEntry {
+  u32 partner;  // the other row; bit 31 set: r is the one not preferred
+  u32 pair;
+};
+struct PairPlan {
+  u64 rows = 0, pairs = 0;
+  int device = 0;
+  DevBuf<u32> off;
+  DevBuf<PairEntry> entry;
+};
+// Checks the pairs (device, [pairs][2]: preferred row, other row) and lays
+// them out; waits for `s`.  Throws when a pair names a row outside
+// [0, rows) or one row twice.
+void build_pair_plan(PairPlan& plan, u64 rows, const i32* pair_rows, u64 pairs, cudaStream_t s);
+void launch_pair_loss(const PairPlan& p, const PairLoss& a, cudaStream_t s);
+
+}  // namespace dp

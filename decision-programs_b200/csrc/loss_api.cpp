@@ -1,0 +1,202 @@
+// extern "C" entry points of the choice losses (declared in
+// include/dp_gbdt.h): argument checks on the host, then asynchronous launches
+// on the caller's stream.
+#include <cmath>
+#include <memory>
+
+#include "../../include/dp_gbdt.h"
+#include "loss.h"
+
+namespace {
+
+using dp::need;
+using dp::u64;
+
+// The C boundary: no exception leaves it, not even one of building a message.
+template <class F>
+int guarded(F&& body) noexcept {
+  try {
+    body();
+    return 0;
+  } catch (const std::exception& e) {
+    try {
+      dp::set_last_error(e.what());
+    } catch (...) {
+    }
+  } catch (...) {
+    try {
+      dp::set_last_error("unknown error");
+    } catch (...) {
+    }
+  }
+  return -1;
+}
+
+// Byte range [lo, hi) that rows of `width` elements, `stride` apart, cover.
+struct Span {
+  u64 lo = 0, hi = 0;
+};
+Span span_of(const void* p, u64 rows, u64 width, u64 stride, u64 size) {
+  const u64 lo = reinterpret_cast<std::uintptr_t>(p);
+  return rows && p ? Span{lo, lo + ((rows - 1) * stride + width) * size} : Span{};
+}
+bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+
+void check_rows(u64 rows, u64 width, u64 stride, u64 size, const void* p, const char* what) {
+  const std::string w(what);
+  need(stride >= width, w + " row stride must cover the classes");
+  need(stride <= (u64(1) << 40), w + " row stride out of range");
+  need(rows <= (u64(1) << 62) / 8 / (stride ? stride : 1), w + " size overflows 64-bit byte offsets");
+  need(rows == 0 || p != nullptr, w + " pointer is null");
+  need(reinterpret_cast<std::uintptr_t>(p) % size == 0, w + " pointer is not aligned to its type");
+}
+
+dp::Margins margins_of(int32_t dtype, const void* margin, u64 rows, uint32_t classes, u64 stride) {
+  need(dtype >= 0 && dtype <= 2, "margin type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+  need(classes >= 1 && classes <= 0x7fffffffu, "the number of classes must be in [1, 2^31)");
+  check_rows(rows, classes, stride, dp::margin_bytes(dtype), margin, "margin");
+  return dp::Margins{margin, dtype, rows, classes, stride};
+}
+
+dp::MarginGrad grad_of(const dp::Margins& m, void* grad, u64 grad_stride, float* hess, u64 hess_stride) {
+  dp::MarginGrad g{};
+  if (!grad) {
+    need(!hess, "the curvature is written with a gradient: the gradient pointer is null");
+    return g;
+  }
+  const u64 size = dp::margin_bytes(m.dtype);
+  check_rows(m.rows, m.classes, grad_stride, size, grad, "gradient");
+  const Span z = span_of(m.z, m.rows, m.classes, m.stride, size),
+             o = span_of(grad, m.rows, m.classes, grad_stride, size);
+  need(!overlap(z, o) || (grad == m.z && grad_stride == m.stride),
+       "the gradient may take the margins' place (same pointer and row stride) but not overlap them otherwise");
+  if (hess) {
+    check_rows(m.rows, m.classes, hess_stride, sizeof(float), hess, "curvature");
+    const Span h = span_of(hess, m.rows, m.classes, hess_stride, sizeof(float));
+    need(!overlap(h, z) && !overlap(h, o), "the curvature overlaps the margins or the gradient");
+  }
+  g.grad = grad;
+  g.grad_stride = grad_stride;
+  g.hess = hess;
+  g.hess_stride = hess_stride;
+  return g;
+}
+
+dp::PairLoss pair_args(const float* score, const float* ref, const float* weight, float beta, float smoothing,
+                       float* loss, float* grad, float* hess, u64 rows, u64 pairs) {
+  need(std::isfinite(beta) && beta > 0.f, "beta must be positive and finite");
+  need(smoothing >= 0.f && smoothing <= 0.5f, "label smoothing must be in [0, 0.5]");
+  need(rows == 0 || (score != nullptr && grad != nullptr), "score or gradient pointer is null");
+  need(pairs == 0 || loss != nullptr, "loss pointer is null");
+  dp::PairLoss a{};
+  a.score = score;
+  a.ref = ref;
+  a.weight = weight;
+  a.beta = beta;
+  a.smoothing = smoothing;
+  a.loss = loss;
+  a.grad = grad;
+  a.hess = hess;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dp_log_prob(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
+                const int32_t* label, float* log_prob, float* norm, void* stream) {
+  return guarded([&] {
+    const dp::Margins m = margins_of(dtype, margin, rows, classes, row_stride);
+    need(rows == 0 || (label != nullptr && log_prob != nullptr && norm != nullptr),
+         "label, log-probability or norm pointer is null");
+    need(reinterpret_cast<std::uintptr_t>(norm) % sizeof(float2) == 0, "norm pointer is not aligned to 8 bytes");
+    dp::launch_log_prob(m, label, log_prob, reinterpret_cast<float2*>(norm), static_cast<cudaStream_t>(stream));
+  });
+}
+
+int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
+                     const int32_t* label, const float* norm, const float* weight, void* grad, uint64_t grad_stride,
+                     float* hess, uint64_t hess_stride, void* stream) {
+  return guarded([&] {
+    const dp::Margins m = margins_of(dtype, margin, rows, classes, row_stride);
+    need(rows == 0 || (label != nullptr && norm != nullptr && weight != nullptr && grad != nullptr),
+         "label, norm, weight or gradient pointer is null");
+    need(reinterpret_cast<std::uintptr_t>(norm) % sizeof(float2) == 0, "norm pointer is not aligned to 8 bytes");
+    const dp::MarginGrad g = grad_of(m, grad, grad_stride, hess, hess_stride);
+    dp::launch_log_prob_grad(m, label, reinterpret_cast<const float2*>(norm), weight, g,
+                             static_cast<cudaStream_t>(stream));
+  });
+}
+
+int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
+                   const int32_t* label, const float* old_log_prob, const float* ref_log_prob,
+                   const float* advantage, const float* weight, float clip_low, float clip_high, float kl,
+                   float* loss, float* log_prob, void* grad, uint64_t grad_stride, float* hess,
+                   uint64_t hess_stride, void* stream) {
+  return guarded([&] {
+    const dp::Margins m = margins_of(dtype, margin, rows, classes, row_stride);
+    need(rows == 0 || (label != nullptr && old_log_prob != nullptr && advantage != nullptr),
+         "label, old log-probability or advantage pointer is null");
+    need(rows == 0 || (loss != nullptr && log_prob != nullptr), "loss or log-probability pointer is null");
+    need(clip_low >= 0.f && clip_low <= 1.f, "clip_low must be in [0, 1]");
+    need(std::isfinite(clip_high) && clip_high >= 0.f, "clip_high must be finite and not negative");
+    need(std::isfinite(kl) && kl >= 0.f, "the KL coefficient must be finite and not negative");
+    const dp::MarginGrad g = grad_of(m, grad, grad_stride, hess, hess_stride);
+    dp::PolicyRows p{};
+    p.old_log_prob = old_log_prob;
+    p.ref_log_prob = ref_log_prob;
+    p.advantage = advantage;
+    p.weight = weight;
+    p.clip_low = clip_low;
+    p.clip_high = clip_high;
+    p.kl = kl;
+    dp::launch_policy_loss(m, label, p, loss, log_prob, g, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int dp_preference_loss(uint64_t rows, const int64_t* item_begin, uint64_t pairs, const float* score,
+                       const float* ref_score, const float* weight, float beta, float smoothing, float* loss,
+                       float* grad, float* hess, void* stream) {
+  return guarded([&] {
+    need(rows < (u64(1) << 60) && pairs < (u64(1) << 40), "rows or pairs out of range");
+    need(item_begin != nullptr || rows >= 2 * pairs, "without item offsets every pair needs two rows");
+    const dp::PairLoss a =
+        pair_args(score, ref_score, weight, beta, smoothing, loss, grad, hess, rows, pairs);
+    dp::launch_preference(a, rows, item_begin, pairs, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int dp_preference_prepare(uint64_t rows, const int32_t* pair_rows, uint64_t pairs, void* stream, void** out_plan) {
+  return guarded([&] {
+    need(out_plan != nullptr, "output pointer is null");
+    need(rows < (u64(1) << 31) && pairs < (u64(1) << 31), "rows and pairs must be below 2^31");
+    need(pairs == 0 || pair_rows != nullptr, "pair pointer is null");
+    auto plan = std::make_unique<dp::PairPlan>();
+    dp::build_pair_plan(*plan, rows, pair_rows, pairs, static_cast<cudaStream_t>(stream));
+    *out_plan = plan.release();
+  });
+}
+
+int dp_preference_run(void* plan, const float* score, const float* ref_score, const float* weight, float beta,
+                      float smoothing, float* loss, float* grad, float* hess, void* stream) {
+  return guarded([&] {
+    need(plan != nullptr, "plan is null");
+    const dp::PairPlan& p = *static_cast<dp::PairPlan*>(plan);
+    const dp::PairLoss a =
+        pair_args(score, ref_score, weight, beta, smoothing, loss, grad, hess, p.rows, p.pairs);
+    dp::DeviceGuard g(p.device);
+    dp::launch_pair_loss(p, a, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int dp_preference_free(void* plan) {
+  return guarded([&] {
+    if (!plan) return;
+    dp::PairPlan* p = static_cast<dp::PairPlan*>(plan);
+    dp::DeviceGuard g(p->device);
+    delete p;
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,95 @@
+// Scalar parts of the choice losses, shared by their kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "loss.h"
+
+namespace dp {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+// A row whose classes are all masked (every margin -inf) has m = -inf and no
+// sum; exponents are then taken relative to 0, so that the sum is 0 and not
+// NaN, and a NaN margin still makes it NaN.
+__device__ __forceinline__ float exp_base(float m) { return m == neg_inf() ? 0.f : m; }
+
+// Log-probability and its two-part norm of a row from its maximum m, the sum
+// s of exp(z - exp_base(m)) and the label's margin.  The norm stays in two
+// parts because exp((z - m) - log s) keeps its precision at margins far from
+// zero, where m + log s would round away what log s says.
+__device__ __forceinline__ float row_log_prob(float m, float s, float zy, float2& norm) {
+  if (s == 0.f) {  // no class left
+    norm = make_float2(neg_inf(), 0.f);
+    return neg_inf();
+  }
+  const float ls = logf(s);
+  norm = make_float2(m, ls);
+  return (zy - m) - ls;
+}
+
+// Clipped policy loss of a row and its derivative by the log-probability:
+// L = w (-min(r A, clamp(r, 1 - lo, 1 + hi) A) + kl (e^d - d - 1)),
+// r = exp(l - old), d = ref - l.  Comparisons keep a NaN ratio NaN.
+__device__ __forceinline__ float policy_row(const PolicyRows& p, u64 r, float l, float& loss) {
+  const float w = p.weight ? p.weight[r] : 1.f;
+  if (w == 0.f) {
+    loss = 0.f;
+    return 0.f;
+  }
+  const float ratio = expf(l - p.old_log_prob[r]), adv = p.advantage[r];
+  const float low = 1.f - p.clip_low, high = 1.f + p.clip_high;
+  const float held = ratio < low ? low : (ratio > high ? high : ratio);
+  const float s1 = ratio * adv, s2 = held * adv;
+  const bool clipped = s1 > s2;
+  float v = clipped ? -s2 : -s1;
+  float c = clipped ? 0.f : -s1;
+  if (p.ref_log_prob) {
+    const float d = p.ref_log_prob[r] - l, e = expm1f(d);
+    v = v + p.kl * (e - d);
+    c = c - p.kl * e;
+  }
+  loss = w * v;
+  return w * c;
+}
+
+// Gradient and curvature of c * log p(label) by one margin of probability p.
+__device__ __forceinline__ float margin_grad(float c, float p, bool chosen) { return c * ((chosen ? 1.f : 0.f) - p); }
+// The softmax objective's diagonal form, with its factor 2 and its floor.
+__device__ __forceinline__ float margin_hess(float c, float p) {
+  return fabsf(c) * fmaxf(2.f * p * (1.f - p), 1e-16f);
+}
+
+// Preference loss of a pair at x = beta * (gap of scores): the loss, its
+// derivative and its second derivative by x.  Both sigmoids come from
+// e = exp(-|x|), which never overflows and keeps a saturated pair's small one.
+struct PairTerms {
+  float loss, slope, bend;
+};
+__device__ __forceinline__ PairTerms pair_terms(float x, float smoothing) {
+  const float e = expf(-fabsf(x)), small = log1pf(e), inv = 1.f / (1.f + e);
+  const float up = x >= 0.f ? inv : e * inv, down = x >= 0.f ? e * inv : inv;  // sigma(x), sigma(-x)
+  const float keep = 1.f - smoothing;
+  PairTerms t;
+  t.loss = keep * (fmaxf(-x, 0.f) + small);
+  if (smoothing != 0.f) t.loss += smoothing * (fmaxf(x, 0.f) + small);  // an infinite x would make 0 * inf of it
+  t.slope = smoothing * up - keep * down;
+  t.bend = up * down;
+  return t;
+}
+// Curvature of an item over its pairs, with the objectives' floor.
+__device__ __forceinline__ float item_hess(float h) { return h < 1e-16f ? 1e-16f : h; }
+
+}  // namespace dp

@@ -14,7 +14,7 @@ import ctypes as C
 import json
 import math
 import pathlib
-from typing import Iterable
+from typing import Any, Iterable, NamedTuple
 
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libdp_gbdt.so"
@@ -24,12 +24,14 @@ EXPORTED = [
     "XGDMatrixCreateFromDense",
     "XGDMatrixSetInfoFromInterface", "XGDMatrixSetFloatInfo", "XGDMatrixNumRow", "XGDMatrixNumCol",
     "XGDMatrixFree", "XGBoosterCreate", "XGBoosterFree", "XGBoosterSetParam", "XGBoosterUpdateOneIter",
-    "XGBoosterBoostedRounds", "XGBoosterSaveJsonConfig", "XGBoosterSaveModel", "XGBoosterSaveModelToBuffer",
+    "XGBoosterTrainOneIter", "XGBoosterBoostedRounds", "XGBoosterSaveJsonConfig", "XGBoosterSaveModel", "XGBoosterSaveModelToBuffer",
     "XGBoosterLoadModelFromBuffer", "XGBoosterLoadModel", "XGBoosterSlice", "XGBoosterGetNumFeature",
     "XGBoosterPredictFromCudaArray",
     "dp_comm_unique_id", "dp_comm_create", "dp_comm_free", "dp_comm_set_timeout", "dp_comm_reduce_scatter_hist", "dp_release_cached_memory", "dp_booster_set_comm", "dp_booster_set_profiling",
-    "dp_booster_profile", "dp_booster_margins", "dp_launch_count", "dp_quantile_cuts", "dp_bin_matrix",
+    "dp_booster_profile", "dp_booster_margins", "dp_booster_train_margin", "dp_launch_count", "dp_quantile_cuts", "dp_bin_matrix",
     "dp_gradients", "dp_hist_build", "dp_hist_build_noalloc", "dp_probe_hist_atomics", "dp_csv_decode", "dp_csv_shape", "dp_csv_data", "dp_csv_metadata", "dp_csv_copy", "dp_csv_free", "dp_csv_parse_feature", "dp_quantize_gh", "dp_hist_prepare", "dp_hist_run", "dp_hist_free", "dp_eval_splits",
+    "dp_log_prob", "dp_log_prob_grad", "dp_policy_loss", "dp_preference_loss", "dp_preference_prepare",
+    "dp_preference_run", "dp_preference_free",
 ]
 
 OBJECTIVE_IDS = {"reg:squarederror": 0, "binary:logistic": 1, "multi:softprob": 2, "multi:softmax": 3}
@@ -65,6 +67,8 @@ def lib() -> C.CDLL:
         L.XGBoosterFree.argtypes = [P]
         L.XGBoosterSetParam.argtypes = [P, C.c_char_p, C.c_char_p]
         L.XGBoosterUpdateOneIter.argtypes = [P, i32, P]
+        L.XGBoosterTrainOneIter.argtypes = [P, P, i32, C.c_char_p, C.c_char_p]
+        L.dp_booster_train_margin.argtypes = [P, P, C.POINTER(u64), C.POINTER(u64), C.POINTER(P)]
         L.XGBoosterBoostedRounds.argtypes = [P, C.POINTER(i32)]
         L.XGBoosterSaveJsonConfig.argtypes = [P, C.POINTER(u64), C.POINTER(C.c_char_p)]
         L.XGBoosterSaveModel.argtypes = [P, C.c_char_p]
@@ -107,6 +111,15 @@ def lib() -> C.CDLL:
         L.dp_hist_run.argtypes = [P, P]
         L.dp_hist_free.argtypes = [P]
         L.dp_eval_splits.argtypes = [P, C.c_int32, C.c_uint32, P, P, P, f32, f32, f64, f64, f64, f64, P, P, P]
+        u32 = C.c_uint32
+        margins = [C.c_int32, P, u64, u32, u64]
+        L.dp_log_prob.argtypes = margins + [P, P, P, P]
+        L.dp_log_prob_grad.argtypes = margins + [P, P, P, P, u64, P, u64, P]
+        L.dp_policy_loss.argtypes = margins + [P, P, P, P, P, f32, f32, f32, P, P, P, u64, P, u64, P]
+        L.dp_preference_loss.argtypes = [u64, P, u64, P, P, P, f32, f32, P, P, P, P]
+        L.dp_preference_prepare.argtypes = [u64, P, u64, P, C.POINTER(P)]
+        L.dp_preference_run.argtypes = [P, P, P, P, f32, f32, P, P, P, P]
+        L.dp_preference_free.argtypes = [P]
         _lib = L
     return _lib
 
@@ -241,6 +254,34 @@ class Booster:
 
     def update(self, dtrain: DMatrix, iteration: int) -> None:
         check(lib().XGBoosterUpdateOneIter(self.handle, iteration, dtrain.handle))
+
+    def boost(self, dtrain: DMatrix, iteration: int, grad, hess) -> None:
+        """One round on the caller's gradients and curvatures: CUDA float32
+        [rows, outputs] (one output: also [rows]), rows strided as they are."""
+        import torch
+        _need(grad.is_cuda and hess.is_cuda and grad.dtype == hess.dtype == torch.float32,
+              "grad and hess must be CUDA float32 tensors")
+        text = [array_interface(t.data_ptr(), list(t.shape), strides=[s * 4 for s in t.stride()]).encode()
+                for t in (grad, hess)]
+        check(lib().XGBoosterTrainOneIter(self.handle, dtrain.handle, iteration, *text))
+
+    def train_margin(self, dtrain: DMatrix):
+        """The training margins of `dtrain` ([rows, outputs] fp32) as a new
+        CUDA tensor: the base scores before the first round."""
+        import torch
+        rows, outputs, ptr = C.c_uint64(), C.c_uint64(), C.c_void_p()
+        check(lib().dp_booster_train_margin(self.handle, dtrain.handle, C.byref(rows), C.byref(outputs),
+                                            C.byref(ptr)))
+
+        class Borrowed:
+            __cuda_array_interface__ = {"data": (ptr.value or 0, False), "shape": (rows.value, outputs.value),
+                                        "typestr": "<f4", "version": 3}
+        if not rows.value:
+            return torch.empty((0, outputs.value), dtype=torch.float32, device="cuda")
+        view = torch.as_tensor(Borrowed())
+        out = view.clone()
+        torch.cuda.current_stream(view.device).synchronize()  # the booster's next call may change them
+        return out
 
     def boosted_rounds(self) -> int:
         n = C.c_int()
@@ -406,6 +447,224 @@ class CsvTable:
         if self.handle:
             check(lib().dp_csv_free(self.handle))
             self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+# ---- losses that learn from choices ------------------------------------------
+# Each call runs on the current torch stream of its tensors' device and returns
+# new tensors; nothing waits for the GPU (PreferencePairs' construction aside).
+
+class PolicyLoss(NamedTuple):
+    """loss and log_prob [R] fp32; grad [R, K] of the margins' type and hess
+    [R, K] fp32, each None when not asked for."""
+    loss: Any
+    log_prob: Any
+    grad: Any
+    hess: Any
+
+
+class PreferenceLoss(NamedTuple):
+    """loss [P], grad [R] and hess [R] (None when not asked for), all fp32."""
+    loss: Any
+    grad: Any
+    hess: Any
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise DPError(message)
+
+
+def _vector(t, n: int, dtype, device, name: str, optional: bool = False, shape=None):
+    """`t` as a contiguous tensor of n rows on `device`, checked."""
+    if t is None and optional:
+        return None
+    shape = (n,) if shape is None else shape
+    _need(tuple(t.shape) == shape, f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+    _need(t.device == device, f"{name} must be on {device}, got {t.device}")
+    return t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class _on:
+    """The device of a call's tensors made current, and its torch stream."""
+
+    def __init__(self, device):
+        import torch
+        _need(device.type == "cuda", "the tensors must be CUDA tensors")
+        self._guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+        self.stream = torch.cuda.current_stream(device).cuda_stream
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+        return self.stream
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _rows_of(t, name: str):
+    """(pointer, row stride) of a [R, K] tensor whose classes are adjacent."""
+    rows, classes = t.shape
+    _need(classes <= 1 or t.stride(1) == 1, f"{name}: the classes of a row must be adjacent in memory")
+    return t.data_ptr(), (t.stride(0) if rows > 1 else max(classes, t.stride(0)))
+
+
+def _margins(margin):
+    """The leading arguments of a call on class margins [R, K]."""
+    import torch
+    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    _need(margin.dim() == 2, "margin must be [rows, classes]")
+    _need(margin.dtype in types, "margin must be float32, float16 or bfloat16")
+    ptr, stride = _rows_of(margin, "margin")
+    return types[margin.dtype], ptr, margin.shape[0], margin.shape[1], stride
+
+
+def _grad_out(margin, grad, hess):
+    """The gradient and curvature tensors of a call, and their arguments."""
+    import torch
+    if grad is None or grad is True:
+        grad = torch.empty(margin.shape, dtype=margin.dtype, device=margin.device)
+    else:
+        _need(grad.shape == margin.shape and grad.dtype == margin.dtype and grad.device == margin.device,
+              "grad must have the margins' shape, type and device")
+    hess = torch.empty(margin.shape, dtype=torch.float32, device=margin.device) if hess else None
+    return grad, hess, (*_rows_of(grad, "grad"), *(_rows_of(hess, "hess") if hess is not None else (None, 0)))
+
+
+def log_prob(margin, label):
+    """log softmax(margin)[label] of every row ([R] fp32), and the rows' norm
+    ([R, 2] fp32: maximum, log-sum) that log_prob_grad takes.  margin: CUDA
+    [R, K] float32, float16 or bfloat16 (row stride allowed); label: int32
+    [R], rows whose label is not a class are skipped."""
+    import torch
+    m = _margins(margin)
+    rows, dev = margin.shape[0], margin.device
+    with _on(dev) as stream:
+        label = _vector(label, rows, torch.int32, dev, "label")
+        out = torch.empty(rows, dtype=torch.float32, device=dev)
+        norm = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+        check(lib().dp_log_prob(*m, label.data_ptr(), out.data_ptr(), norm.data_ptr(), stream))
+    return out, norm
+
+
+def log_prob_grad(margin, label, norm, weight, grad=None, hess: bool = False):
+    """The backward pass of log_prob: (grad, hess) for `weight` [R] fp32, the
+    derivative of a loss by each log-probability.  grad: a tensor to write to
+    (the margins themselves included); hess: the diagonal curvature too."""
+    import torch
+    m = _margins(margin)
+    rows, dev = margin.shape[0], margin.device
+    with _on(dev) as stream:
+        label = _vector(label, rows, torch.int32, dev, "label")
+        norm = _vector(norm, rows, torch.float32, dev, "norm", shape=(rows, 2))
+        weight = _vector(weight, rows, torch.float32, dev, "weight")
+        grad, hess, out = _grad_out(margin, grad, hess)
+        check(lib().dp_log_prob_grad(*m, label.data_ptr(), norm.data_ptr(), weight.data_ptr(), *out, stream))
+    return grad, hess
+
+
+def policy_loss(margin, label, old_log_prob, advantage, ref_log_prob=None, weight=None, clip=(0.2, 0.2),
+                kl: float = 0.0, grad=True, hess: bool = False) -> PolicyLoss:
+    """Clipped policy loss with a KL term (dp_policy_loss): margin [R, K] as in
+    log_prob, label the sampled class; old_log_prob, advantage, ref_log_prob
+    (None: no KL term) and weight (None: 1) [R] fp32; clip (low, high).  grad:
+    True, a tensor to write to (the margins themselves included), or False for
+    the forward pass alone; hess: the diagonal curvature too."""
+    import torch
+    m = _margins(margin)
+    rows, dev = margin.shape[0], margin.device
+    with _on(dev) as stream:
+        label = _vector(label, rows, torch.int32, dev, "label")
+        old_log_prob = _vector(old_log_prob, rows, torch.float32, dev, "old_log_prob")
+        advantage = _vector(advantage, rows, torch.float32, dev, "advantage")
+        ref_log_prob = _vector(ref_log_prob, rows, torch.float32, dev, "ref_log_prob", optional=True)
+        weight = _vector(weight, rows, torch.float32, dev, "weight", optional=True)
+        _need(grad is not False or not hess, "hess is written with a gradient: grad is False")
+        loss = torch.empty(rows, dtype=torch.float32, device=dev)
+        logp = torch.empty(rows, dtype=torch.float32, device=dev)
+        grad, hess, out = (None, None, (None, 0, None, 0)) if grad is False else _grad_out(margin, grad, hess)
+        check(lib().dp_policy_loss(*m, label.data_ptr(), old_log_prob.data_ptr(), _ptr(ref_log_prob),
+                                   advantage.data_ptr(), _ptr(weight), clip[0], clip[1], kl, loss.data_ptr(),
+                                   logp.data_ptr(), *out, stream))
+    return PolicyLoss(loss, logp, grad, hess)
+
+
+def _pair_tensors(score, ref_score, weight, pairs: int, hess: bool):
+    import torch
+    _need(score.dim() == 1, "score must be a vector")
+    rows, dev = score.shape[0], score.device
+    score = _vector(score, rows, torch.float32, dev, "score")
+    ref_score = _vector(ref_score, rows, torch.float32, dev, "ref_score", optional=True)
+    weight = _vector(weight, pairs, torch.float32, dev, "weight", optional=True)
+    new = lambda n: torch.empty(n, dtype=torch.float32, device=dev)  # noqa: E731
+    return score, ref_score, weight, PreferenceLoss(new(pairs), new(rows), new(rows) if hess else None)
+
+
+def preference_loss(score, ref_score=None, item_begin=None, weight=None, beta: float = 1.0, smoothing: float = 0.0,
+                    hess: bool = False) -> PreferenceLoss:
+    """Preference loss over consecutive items (dp_preference_loss): item 2p is
+    preferred to item 2p + 1.  score, ref_score: [R] fp32 CUDA; item_begin:
+    int64 [2P + 1] offsets into the rows (None: every row is an item); weight:
+    [P] fp32."""
+    import torch
+    dev = score.device
+    with _on(dev) as stream:
+        if item_begin is None:
+            _need(score.dim() == 1 and score.shape[0] % 2 == 0, "without item offsets score holds pairs of rows")
+            pairs = score.shape[0] // 2
+        else:
+            _need(item_begin.dim() == 1 and item_begin.shape[0] % 2 == 1, "item_begin must hold 2 * pairs + 1 offsets")
+            pairs = item_begin.shape[0] // 2
+            item_begin = _vector(item_begin, 2 * pairs + 1, torch.int64, dev, "item_begin")
+        score, ref_score, weight, out = _pair_tensors(score, ref_score, weight, pairs, hess)
+        check(lib().dp_preference_loss(score.shape[0], _ptr(item_begin), pairs, score.data_ptr(), _ptr(ref_score),
+                                       _ptr(weight), beta, smoothing, out.loss.data_ptr(), out.grad.data_ptr(),
+                                       _ptr(out.hess), stream))
+    return out
+
+
+class PreferencePairs:
+    """Pairs of rows, checked and laid out once (dp_preference_prepare): pairs
+    [P, 2] int32 CUDA (preferred row, other row) over `rows` rows; a row may be
+    in any number of pairs."""
+
+    def __init__(self, pairs, rows: int):
+        import torch
+        self.handle = C.c_void_p()
+        self.pairs, self.rows, self.device = pairs.shape[0], int(rows), pairs.device
+        with _on(pairs.device) as stream:
+            pairs = _vector(pairs, self.pairs, torch.int32, pairs.device, "pairs", shape=(self.pairs, 2))
+            check(lib().dp_preference_prepare(self.rows, pairs.data_ptr(), self.pairs, stream, C.byref(self.handle)))
+
+    def loss(self, score, ref_score=None, weight=None, beta: float = 1.0, smoothing: float = 0.0,
+             hess: bool = False) -> PreferenceLoss:
+        """The preference loss of score [rows] fp32, with weight [P]."""
+        _need(bool(self.handle), "the pairs have been freed")
+        _need(tuple(score.shape) == (self.rows,), f"score must have shape {[self.rows]}, got {list(score.shape)}")
+        _need(score.device == self.device, f"score must be on {self.device}, got {score.device}")
+        with _on(self.device) as stream:
+            score, ref_score, weight, out = _pair_tensors(score, ref_score, weight, self.pairs, hess)
+            check(lib().dp_preference_run(self.handle, score.data_ptr(), _ptr(ref_score), _ptr(weight), beta,
+                                          smoothing, out.loss.data_ptr(), out.grad.data_ptr(), _ptr(out.hess),
+                                          stream))
+        return out
+
+    def free(self) -> None:
+        if self.handle:
+            check(lib().dp_preference_free(self.handle))
+            self.handle = C.c_void_p()
 
     def __del__(self):
         try:

@@ -85,6 +85,17 @@ DP_API int XGBoosterSetParam(BoosterHandle handle, const char* name, const char*
  * The hot path: replaces native/class_native_training.cuh:67. */
 DP_API int XGBoosterUpdateOneIter(BoosterHandle handle, int iter, DMatrixHandle dtrain);
 
+/* One boosting round on the caller's gradients and curvatures (array
+ * interfaces: fp32 CUDA memory on the matrix's device, [rows, outputs] with a
+ * row's outputs adjacent, or [rows] for one output); the objective then only
+ * names the outputs and the prediction's transform, and the matrix needs no
+ * labels.  Waits for the device's earlier work, and is synchronous like
+ * XGBoosterUpdateOneIter; rounds of both kinds may alternate.  Values that are
+ * not finite and negative curvatures are refused and leave the model as it
+ * was.  XGBoost C API function; the reference does not bind it. */
+DP_API int XGBoosterTrainOneIter(BoosterHandle handle, DMatrixHandle dtrain, int iter, const char* grad,
+                                 const char* hess);
+
 /* native/class_model_train.cu:49, native/class_study_train.cu:104,127,328. */
 DP_API int XGBoosterBoostedRounds(BoosterHandle handle, int* out);
 
@@ -171,6 +182,14 @@ DP_API int dp_booster_profile(BoosterHandle handle, const char** out_json);
 
 /* Training margins [R][K] of the booster's training matrix (host copy). */
 DP_API int dp_booster_margins(BoosterHandle handle, float* out, bst_ulong len);
+
+/* The training margins on the device, [rows][outputs] fp32: what a loss of
+ * the caller's is evaluated on between rounds.  Binds the booster to the
+ * matrix as a training call does (before the first round they are the base
+ * scores).  Borrowed and read-only; valid until the next call on the booster,
+ * which must not start before the caller's work that reads them has ended. */
+DP_API int dp_booster_train_margin(BoosterHandle handle, DMatrixHandle dtrain, bst_ulong* out_rows,
+                                   bst_ulong* out_outputs, const float** out);
 
 /* Number of CUDA kernels this library has launched in the process. */
 DP_API uint64_t dp_launch_count(void);
@@ -272,6 +291,77 @@ DP_API int dp_eval_splits(const int64_t* hist, int32_t nnodes, uint32_t features
                           const uint8_t* has_missing, const int64_t* totals, float sg, float sh, double lambda,
                           double alpha, double gamma, double min_child_weight, int32_t* out_i, double* out_gain,
                           int64_t* out_left);
+
+/* ---- losses that learn from choices ---------------------------------------
+ * Log-probabilities of a chosen class, the clipped policy loss and the
+ * preference loss, each with its gradient; no counterpart in the reference,
+ * whose trainer has one fixed objective.  Device pointers throughout; work is
+ * ordered on `stream` of the calling thread's current device and nothing is
+ * allocated or waited for (dp_preference_prepare aside).  Results do not
+ * change from run to run.  A gradient and its curvature are what
+ * XGBoosterTrainOneIter takes.
+ *
+ * margin: [rows][classes] of `dtype` 0 fp32, 1 fp16 or 2 bf16, rows
+ * `row_stride` elements apart, any alignment of the type.  Sums and
+ * exponentials are fp32; a gradient is rounded to `dtype` once.
+ *  - label (int32) outside [0, classes): the row is skipped: its margins are
+ *    not read, its outputs and its gradient row are 0.
+ *  - margins of -inf are masked classes of probability 0.  A row that masks
+ *    every class has log-probability -inf, loss 0 and a zero gradient.
+ *  - NaN or +inf in a row that is not skipped makes that row's results NaN,
+ *    and no other's. */
+
+/* log_prob[rows] = log softmax(margin)[label], and norm[rows][2] = (maximum,
+ * log of the sum of exp(margin - maximum)), which dp_log_prob_grad reads. */
+DP_API int dp_log_prob(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
+                       const int32_t* label, float* log_prob, float* norm, void* stream);
+/* The backward pass: grad[rows][classes] (of `dtype`) = weight[r] *
+ * ([k == label] - p_k), weight being the derivative of a loss by log_prob[r];
+ * hess (fp32, may be NULL) = |weight[r]| * max(2 p_k (1 - p_k), 1e-16), the
+ * softmax objective's diagonal form.  weight 0: the row's margins are not read
+ * and its outputs are 0.  grad may be margin itself (same row stride);
+ * other overlaps are refused. */
+DP_API int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
+                            const int32_t* label, const float* norm, const float* weight, void* grad,
+                            uint64_t grad_stride, float* hess, uint64_t hess_stride, void* stream);
+/* Clipped policy loss with a KL term, forward and backward in one pass:
+ * l = log softmax(margin)[label], r = exp(l - old_log_prob), d = ref_log_prob - l,
+ * loss[rows] = weight * (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *                        + kl (exp(d) - d - 1)),
+ * A the advantage.  ref_log_prob NULL: no KL term; weight NULL: 1; weight 0:
+ * loss and gradient row are 0 whatever the row holds.  log_prob[rows]
+ * receives l.  grad / hess as in dp_log_prob_grad with the loss's derivative
+ * by l for its weight; grad NULL: the forward pass alone. */
+DP_API int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
+                          const int32_t* label, const float* old_log_prob, const float* ref_log_prob,
+                          const float* advantage, const float* weight, float clip_low, float clip_high, float kl,
+                          float* loss, float* log_prob, void* grad, uint64_t grad_stride, float* hess,
+                          uint64_t hess_stride, void* stream);
+/* Preference loss over paired items.  Item i is rows [item_begin[i],
+ * item_begin[i + 1]) of score (int64 offsets, 2 * pairs + 1 of them,
+ * ascending; an item may be empty, offsets past the rows are taken as their
+ * end), or row i when item_begin is NULL.  Pair p prefers item 2p to
+ * item 2p + 1: x = beta ((S_2p - S_2p+1) - (T_2p - T_2p+1)), S the item's sum
+ * of score and T its sum of ref_score (NULL: 0),
+ * loss[pairs] = weight ((1 - smoothing) softplus(-x) + smoothing softplus(x)).
+ * grad[rows] is its derivative by every score (all rows of an item share it),
+ * hess[rows] (may be NULL) the second one, at least 1e-16; rows outside every
+ * item get 0 (1e-16).  weight (per pair) NULL: 1; weight 0: the pair counts
+ * for nothing, whatever its scores hold. */
+DP_API int dp_preference_loss(uint64_t rows, const int64_t* item_begin, uint64_t pairs, const float* score,
+                              const float* ref_score, const float* weight, float beta, float smoothing, float* loss,
+                              float* grad, float* hess, void* stream);
+/* The same loss over any pairs of rows: pair_rows[pairs][2] (int32, device) =
+ * preferred row, other row; a row may be in any number of pairs, and its
+ * gradient and curvature sum over them.  dp_preference_prepare checks the
+ * pairs (a row out of range or a pair of one row with itself is refused),
+ * lays them out once and waits for `stream`; dp_preference_run then runs on
+ * that layout, which it does not change, so runs of one plan may overlap. */
+DP_API int dp_preference_prepare(uint64_t rows, const int32_t* pair_rows, uint64_t pairs, void* stream,
+                                 void** out_plan);
+DP_API int dp_preference_run(void* plan, const float* score, const float* ref_score, const float* weight, float beta,
+                             float smoothing, float* loss, float* grad, float* hess, void* stream);
+DP_API int dp_preference_free(void* plan);
 
 #ifdef __cplusplus
 }
