@@ -36,11 +36,38 @@ struct PolicyRows {
   float clip_low = 0.f, clip_high = 0.f, kl = 0.f;
 };
 
-void launch_log_prob(const Margins& m, const i32* label, float* log_prob, float2* norm, cudaStream_t s);
-void launch_log_prob_grad(const Margins& m, const i32* label, const float2* norm, const float* weight,
-                          const MarginGrad& out, cudaStream_t s);
-void launch_policy_loss(const Margins& m, const i32* label, const PolicyRows& p, float* loss, float* log_prob,
-                        const MarginGrad& out, cudaStream_t s);
+// Forward (and, for the policy loss, backward) pass over rows: log_prob and
+// norm, or loss, log_prob and the gradient.
+struct RowArgs {
+  Margins m;
+  const i32* label = nullptr;
+  PolicyRows policy;
+  float* loss = nullptr;
+  float* log_prob = nullptr;
+  float2* norm = nullptr;
+  MarginGrad out;
+};
+// The log-probability's backward pass.
+struct GradArgs {
+  Margins m;
+  const i32* label = nullptr;
+  const float2* norm = nullptr;
+  const float* weight = nullptr;
+  MarginGrad out;
+};
+// One source file a margin type.
+void launch_rows_f32(const RowArgs& a, bool policy, cudaStream_t s);
+void launch_rows_f16(const RowArgs& a, bool policy, cudaStream_t s);
+void launch_rows_bf16(const RowArgs& a, bool policy, cudaStream_t s);
+void launch_grad_f32(const GradArgs& a, cudaStream_t s);
+void launch_grad_f16(const GradArgs& a, cudaStream_t s);
+void launch_grad_bf16(const GradArgs& a, cudaStream_t s);
+inline void launch_rows(const RowArgs& a, bool policy, cudaStream_t s) {
+  (a.m.dtype == kF32 ? launch_rows_f32 : a.m.dtype == kF16 ? launch_rows_f16 : launch_rows_bf16)(a, policy, s);
+}
+inline void launch_grad(const GradArgs& a, cudaStream_t s) {
+  (a.m.dtype == kF32 ? launch_grad_f32 : a.m.dtype == kF16 ? launch_grad_f16 : launch_grad_bf16)(a, s);
+}
 
 // Scores of items: item i is rows [begin[i], begin[i + 1]) of score (begin
 // null: row i); pair p is items 2p (preferred) and 2p + 1.

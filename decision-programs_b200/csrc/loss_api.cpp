@@ -111,7 +111,12 @@ int dp_log_prob(int32_t dtype, const void* margin, uint64_t rows, uint32_t class
     need(rows == 0 || (label != nullptr && log_prob != nullptr && norm != nullptr),
          "label, log-probability or norm pointer is null");
     need(reinterpret_cast<std::uintptr_t>(norm) % sizeof(float2) == 0, "norm pointer is not aligned to 8 bytes");
-    dp::launch_log_prob(m, label, log_prob, reinterpret_cast<float2*>(norm), static_cast<cudaStream_t>(stream));
+    dp::RowArgs a{};
+    a.m = m;
+    a.label = label;
+    a.log_prob = log_prob;
+    a.norm = reinterpret_cast<float2*>(norm);
+    dp::launch_rows(a, false, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -124,8 +129,8 @@ int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, uint32_t 
          "label, norm, weight or gradient pointer is null");
     need(reinterpret_cast<std::uintptr_t>(norm) % sizeof(float2) == 0, "norm pointer is not aligned to 8 bytes");
     const dp::MarginGrad g = grad_of(m, grad, grad_stride, hess, hess_stride);
-    dp::launch_log_prob_grad(m, label, reinterpret_cast<const float2*>(norm), weight, g,
-                             static_cast<cudaStream_t>(stream));
+    dp::launch_grad(dp::GradArgs{m, label, reinterpret_cast<const float2*>(norm), weight, g},
+                    static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -142,8 +147,13 @@ int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t cl
     need(clip_low >= 0.f && clip_low <= 1.f, "clip_low must be in [0, 1]");
     need(std::isfinite(clip_high) && clip_high >= 0.f, "clip_high must be finite and not negative");
     need(std::isfinite(kl) && kl >= 0.f, "the KL coefficient must be finite and not negative");
-    const dp::MarginGrad g = grad_of(m, grad, grad_stride, hess, hess_stride);
-    dp::PolicyRows p{};
+    dp::RowArgs a{};
+    a.m = m;
+    a.label = label;
+    a.loss = loss;
+    a.log_prob = log_prob;
+    a.out = grad_of(m, grad, grad_stride, hess, hess_stride);
+    dp::PolicyRows& p = a.policy;
     p.old_log_prob = old_log_prob;
     p.ref_log_prob = ref_log_prob;
     p.advantage = advantage;
@@ -151,7 +161,7 @@ int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t cl
     p.clip_low = clip_low;
     p.clip_high = clip_high;
     p.kl = kl;
-    dp::launch_policy_loss(m, label, p, loss, log_prob, g, static_cast<cudaStream_t>(stream));
+    dp::launch_rows(a, true, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -40,16 +40,20 @@ __device__ __forceinline__ float row_log_prob(float m, float s, float zy, float2
   return (zy - m) - ls;
 }
 
+// What a row's loss reads beside its margins; zy: the label's margin.
+struct RowScalars {
+  float zy = 0.f, old = 0.f, ref = 0.f, adv = 0.f, w = 1.f;
+};
+
 // Clipped policy loss of a row and its derivative by the log-probability:
 // L = w (-min(r A, clamp(r, 1 - lo, 1 + hi) A) + kl (e^d - d - 1)),
 // r = exp(l - old), d = ref - l.  Comparisons keep a NaN ratio NaN.
-__device__ __forceinline__ float policy_row(const PolicyRows& p, u64 r, float l, float& loss) {
-  const float w = p.weight ? p.weight[r] : 1.f;
-  if (w == 0.f) {
+__device__ __forceinline__ float policy_row(const PolicyRows& p, const RowScalars& x, float l, float& loss) {
+  if (x.w == 0.f) {
     loss = 0.f;
     return 0.f;
   }
-  const float ratio = expf(l - p.old_log_prob[r]), adv = p.advantage[r];
+  const float ratio = expf(l - x.old), adv = x.adv;
   const float low = 1.f - p.clip_low, high = 1.f + p.clip_high;
   const float held = ratio < low ? low : (ratio > high ? high : ratio);
   const float s1 = ratio * adv, s2 = held * adv;
@@ -57,12 +61,12 @@ __device__ __forceinline__ float policy_row(const PolicyRows& p, u64 r, float l,
   float v = clipped ? -s2 : -s1;
   float c = clipped ? 0.f : -s1;
   if (p.ref_log_prob) {
-    const float d = p.ref_log_prob[r] - l, e = expm1f(d);
+    const float d = x.ref - l, e = expm1f(d);
     v = v + p.kl * (e - d);
     c = c - p.kl * e;
   }
-  loss = w * v;
-  return w * c;
+  loss = x.w * v;
+  return x.w * c;
 }
 
 // Gradient and curvature of c * log p(label) by one margin of probability p.
