@@ -11,6 +11,7 @@
 // ragged first and last ones element by element, so that nothing outside the
 // row is read or written.
 #pragma once
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -138,21 +139,6 @@ struct MaxOp {
 struct SumOp {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
 };
-// Over the G threads of a row: part of a warp, or the whole block (every
-// thread of it calls; `part` is shared memory of a call of its own).
-template <int G, class Op>
-__device__ __forceinline__ float group_reduce(float v, float* part, Op op) {
-  if constexpr (G <= 32) {
-    return lanes_reduce<G>(v, op);
-  } else {
-    v = lanes_reduce<32>(v, op);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = part[threadIdx.x & (G / 32 - 1)];  // every warp reduces the warps' results alike
-    return lanes_reduce<G / 32>(v, op);
-  }
-}
-
 __device__ __forceinline__ u32 cluster_rank() {
   u32 r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -179,6 +165,7 @@ __device__ __forceinline__ float rebase(float s, float from, float to) {
 // ranks: every block gets the same two numbers.
 __device__ __forceinline__ void cluster_join(float2* parts, u32 blocks, float& m, float& s) {
   if (threadIdx.x < blocks) cluster_put(parts + cluster_rank(), threadIdx.x, make_float2(m, s));
+  __syncwarp();
   cluster_arrive();
   cluster_wait();
   float top = neg_inf();
@@ -260,157 +247,293 @@ __device__ __forceinline__ void zero_vector(const RowCut<T>& cut, u32 j, T* g, f
   if (h) cut.store(h, j, e);
 }
 
-// G threads a row, V vectors a thread; `blocks` blocks of a cluster share a
-// row when G is the whole block.
+// G lanes of a warp a row, V vectors a lane, kept in registers.
 template <class T, bool kPolicy, int G, int V>
-__global__ void __launch_bounds__(G <= 32 ? 256 : G, G <= 256 ? 4 : 2) k_row_loss(RowArgs a, u32 blocks) {
+__global__ void __launch_bounds__(256, 4) k_row_loss(RowArgs a) {
   constexpr int N = Vec<T>::N;
-  constexpr bool kBlock = G > 32;
-  __shared__ float part[2][kBlock ? G / 32 : 1];
-  __shared__ float2 parts[kBlock ? kMaxCluster : 1];
-  const u32 lane = kBlock ? threadIdx.x : threadIdx.x % G;
-  const u32 rank = kBlock && blocks > 1 ? cluster_rank() : 0;
-  if (kBlock && blocks > 1) cluster_arrive();  // (waited for before another block's memory is written)
-  const u64 r = kBlock ? blockIdx.x / blocks : u64(blockIdx.x) * (256 / G) + threadIdx.x / G;
-  const bool in = kBlock || r < a.m.rows;
+  const u32 lane = threadIdx.x % G;
+  const u64 r = u64(blockIdx.x) * (256 / G) + threadIdx.x / G;
+  const bool in = r < a.m.rows;
   const i32 y = in ? a.label[r] : -1;
   const bool live = u32(y) < a.m.classes;
   const RowCut<T> cut(static_cast<const T*>(a.m.z) + (in ? r : 0) * a.m.stride, a.m.classes);
-  const u32 nvec = cut.vectors(), per = kBlock ? (nvec + blocks - 1) / blocks : nvec;
-  const u32 j0 = rank * per, j1 = min(nvec, j0 + per);
-  float c = 0.f, base = 0.f, scale = 0.f;
+  const u32 nvec = cut.vectors();
+  float c = 0.f, base = 0.f, scale = 0.f, m = neg_inf(), s = 0.f;
   Vec<T> v[V];
-  if (live || !kBlock) {  // (the lanes of a warp reduce together, whatever their rows)
-    RowScalars x;
-    float m = neg_inf(), s = 0.f;
-    if (live) {
-      x = policy_scalars<kPolicy>(a, r);
-      x.zy = to_f32(cut.z[y]);
+  RowScalars x;
+  if (live) {
+    x = policy_scalars<kPolicy>(a, r);
+    x.zy = to_f32(cut.z[y]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const u32 j = j0 + lane + i * G;
-        if (j < j1) v[i] = cut.load(j, neg_inf());
-        else v[i].fill(neg_inf());
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float f[N];
-        v[i].unpack(f);
-#pragma unroll
-        for (int k = 0; k < N; ++k) m = fmaxf(m, f[k]);
-      }
+    for (int i = 0; i < V; ++i) {
+      const u32 j = lane + i * G;
+      if (j < nvec) v[i] = cut.load(j, neg_inf());
+      else v[i].fill(neg_inf());
     }
-    m = group_reduce<G>(m, part[0], MaxOp());
-    base = exp_base(m);
-    if (live) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float f[N];
-        v[i].unpack(f);
+    for (int i = 0; i < V; ++i) {
+      float f[N];
+      v[i].unpack(f);
 #pragma unroll
-        for (int k = 0; k < N; ++k) s += exp_fast(f[k] - base);
-      }
+      for (int k = 0; k < N; ++k) m = fmaxf(m, f[k]);
     }
-    s = group_reduce<G>(s, part[1], SumOp());
-    if constexpr (kBlock) {
-      if (blocks > 1) {
-        cluster_wait();
-        cluster_join(parts, blocks, m, s);
-        base = exp_base(m);
-      }
-    }
-    if (live) {
-      c = finish_row<kPolicy>(a, r, x, m, s, rank == 0 && lane == 0);
-      scale = 1.f / s;
-    }
-  } else if (blocks > 1) {
-    cluster_wait();
   }
-  if (in && !live) skip_row<kPolicy>(a, r, rank == 0 && lane == 0);
-  // (a gradient in the margins' place: every lane has read its label's margin)
-  if constexpr (!kBlock) __syncwarp();
+  m = lanes_reduce<G>(m, MaxOp());  // (the lanes of a warp reduce together, whatever their rows)
+  base = exp_base(m);
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float f[N];
+      v[i].unpack(f);
+#pragma unroll
+      for (int k = 0; k < N; ++k) s += exp_fast(f[k] - base);
+    }
+  }
+  s = lanes_reduce<G>(s, SumOp());
+  if (live) {
+    c = finish_row<kPolicy>(a, r, x, m, s, lane == 0);
+    scale = 1.f / s;
+  } else if (in) {
+    skip_row<kPolicy>(a, r, lane == 0);
+  }
+  __syncwarp();  // (a gradient in the margins' place: every lane has read its label's margin)
   if constexpr (kPolicy) {
     if (!a.out.grad || !in) return;
     T* const g = static_cast<T*>(a.out.grad) + r * a.out.grad_stride;
     float* const h = a.out.hess ? a.out.hess + r * a.out.hess_stride : nullptr;
     if (c == 0.f) {
-      for (u32 j = j0 + lane; j < j1; j += G) zero_vector(cut, j, g, h);
+      for (u32 j = lane; j < nvec; j += G) zero_vector(cut, j, g, h);
       return;
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const u32 j = j0 + lane + i * G;
-      if (j < j1) grad_vector(cut, j, v[i], y, c, base, 0.f, scale, g, h);
+      const u32 j = lane + i * G;
+      if (j < nvec) grad_vector(cut, j, v[i], y, c, base, 0.f, scale, g, h);
     }
   }
 }
 
-// Rows too long for registers: `blocks` blocks of a cluster walk their share
-// of the row twice, first for the maximum and the sum (each thread keeps its
-// own running pair), then for the gradient.
-template <class T, bool kPolicy>
-__global__ void __launch_bounds__(512) k_row_loss_long(RowArgs a, u32 blocks) {
-  constexpr int N = Vec<T>::N, G = 512, U = 4;
-  __shared__ float part[2][G / 32];
-  __shared__ float2 parts[kMaxCluster];
-  const u32 rank = cluster_rank();
-  cluster_arrive();
-  const u64 r = blockIdx.x / blocks;
-  const i32 y = a.label[r];
-  const bool live = u32(y) < a.m.classes;
-  const RowCut<T> cut(static_cast<const T*>(a.m.z) + r * a.m.stride, a.m.classes);
-  const u32 nvec = cut.vectors(), per = (nvec + blocks - 1) / blocks;
-  const u32 j0 = min(nvec, rank * per), j1 = min(nvec, j0 + per);
-  float c = 0.f, base = 0.f, scale = 0.f;
-  if (live) {
-    RowScalars x = policy_scalars<kPolicy>(a, r);
-    x.zy = to_f32(cut.z[y]);
-    float m = neg_inf(), s = 0.f;
-    for (u32 j = j0 + threadIdx.x; j < j1; j += U * G) {
-      Vec<T> v[U];
-      float top = m;
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (j + i * G < j1) v[i] = cut.load(j + i * G, neg_inf());
-        else v[i].fill(neg_inf());
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        float f[N];
-        v[i].unpack(f);
-#pragma unroll
-        for (int k = 0; k < N; ++k) top = fmaxf(top, f[k]);
-      }
-      const float b = exp_base(top);
-      s = rebase(s, m, top);
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        float f[N];
-        v[i].unpack(f);
-#pragma unroll
-        for (int k = 0; k < N; ++k) s += exp_fast(f[k] - b);
-      }
-      m = top;
-    }
-    const float mine = m;
-    m = group_reduce<G>(m, part[0], MaxOp());
-    s = group_reduce<G>(rebase(s, mine, m), part[1], SumOp());
-    cluster_wait();
-    cluster_join(parts, blocks, m, s);
-    base = exp_base(m);
-    c = finish_row<kPolicy>(a, r, x, m, s, rank == 0 && threadIdx.x == 0);
-    scale = 1.f / s;
+// ---- long rows --------------------------------------------------------------
+// `blocks` blocks of a cluster share a row, and each cluster walks its rows
+// (r, r + clusters, ...).  Every thread streams its own vectors through its
+// own places of a ring in shared memory, by asynchronous copies that run
+// ahead of it into the following rows, so that margins keep arriving while
+// sums are joined and gradients are written; nothing in the ring is shared,
+// so it needs no barrier.  A row that fits in the ring stays there between
+// its sum and its gradient (one read of the margins); a longer one is
+// streamed twice.
+__device__ __forceinline__ void copy_async(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(u32(__cvta_generic_to_shared(shared))), "l"(global)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most n (below S) of this thread's latest groups are under way.
+template <int S>
+__device__ __forceinline__ void copy_wait(u32 n) {
+  if constexpr (S > 1) {
+    if (n == S - 1) asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+    else copy_wait<S - 1>(n);
   } else {
-    cluster_wait();
-    skip_row<kPolicy>(a, r, rank == 0 && threadIdx.x == 0);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  if constexpr (kPolicy) {
-    if (!a.out.grad) return;
-    T* const g = static_cast<T*>(a.out.grad) + r * a.out.grad_stride;
-    float* const h = a.out.hess ? a.out.hess + r * a.out.hess_stride : nullptr;
-    for (u32 j = j0 + threadIdx.x; j < j1; j += G) {
-      if (c == 0.f) zero_vector(cut, j, g, h);
-      else grad_vector(cut, j, cut.load(j, neg_inf()), y, c, base, 0.f, scale, g, h);
+}
+
+// The rows of one cluster in order, their labels read 32 at a time.
+struct RowWalk {
+  const i32* label;
+  u64 rows, step, r;
+  u32 classes, at = 32;
+  i32 batch = -1;
+  __device__ RowWalk(const RowArgs& a, u64 first, u64 clusters)
+      : label(a.label), rows(a.m.rows), step(clusters), r(first), classes(a.m.classes) {}
+  __device__ bool done() const { return r >= rows; }
+  __device__ i32 here() {
+    if (at == 32) {
+      const u64 mine = r + (threadIdx.x & 31) * step;
+      batch = mine < rows ? label[mine] : -1;
+      at = 0;
+    }
+    return __shfl_sync(0xffffffffu, batch, at);
+  }
+  __device__ void next() {
+    r += step;
+    ++at;
+  }
+};
+
+// One block's share [j0, j1) of a row's vectors, in groups of NT * U.
+template <class T, int NT, int U>
+struct RowShare {
+  u32 j0 = 0, j1 = 0;
+  RowShare() = default;
+  __device__ RowShare(const RowCut<T>& cut, u32 rank, u32 blocks) {
+    const u32 nvec = cut.vectors(), per = (nvec + blocks - 1) / blocks;
+    j0 = min(nvec, rank * per);
+    j1 = min(nvec, j0 + per);
+  }
+  __device__ u32 groups() const { return (j1 - j0 + NT * U - 1) / (NT * U); }
+};
+
+template <class T, bool kPolicy, int NT, int U, int S>
+__global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32 clusters) {
+  constexpr int N = Vec<T>::N, kWarps = NT / 32;
+  extern __shared__ uint4 ring[];  // [S][U][NT]
+  __shared__ float2 warp_part[2][kWarps];
+  __shared__ float2 block_part[2][kMaxCluster];
+  const u32 t = threadIdx.x, rank = blocks > 1 ? cluster_rank() : 0;
+  const u64 first = blockIdx.x / blocks;
+  const T* const z = static_cast<const T*>(a.m.z);
+  if (blocks > 1) {  // every block runs before another one writes to its memory
+    cluster_arrive();
+    cluster_wait();
+  }
+  const bool backward = kPolicy && a.out.grad != nullptr;
+
+  // the copies' place: row, share, next group, and which pass over the row
+  RowWalk in_rows(a, first, clusters);
+  RowCut<T> in_cut(z, a.m.classes);
+  RowShare<T, NT, U> in_share;
+  u32 in_group = 0, in_groups = 0, in_slot = 0;
+  bool again = false;
+  auto issue = [&]() {
+    while (in_group == in_groups && !(in_groups && again) && !in_rows.done()) {
+      const bool live = u32(in_rows.here()) < a.m.classes;
+      if (live) {
+        in_cut = RowCut<T>(z + in_rows.r * a.m.stride, a.m.classes);
+        in_share = RowShare<T, NT, U>(in_cut, rank, blocks);
+        in_group = 0;
+        in_groups = in_share.groups();
+        again = backward && in_groups > S;
+      }
+      in_rows.next();
+    }
+    if (in_group == in_groups && again) {  // the second pass over a row that the ring does not hold
+      in_group = 0;
+      again = false;
+    }
+    if (in_group < in_groups) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const u32 j = in_share.j0 + (in_group * U + u) * NT + t;
+        uint4* const at = ring + (in_slot * U + u) * NT + t;
+        if (j < in_share.j1) {
+          if (in_cut.whole(j)) copy_async(at, in_cut.z + in_cut.first(j));
+          else *at = in_cut.load(j, neg_inf()).raw;
+        }
+      }
+      ++in_group;
+    }
+    copy_commit();  // (empty groups too: the count of groups under way stays S)
+    in_slot = in_slot + 1 == S ? 0 : in_slot + 1;
+  };
+  for (int i = 0; i < S; ++i) issue();
+
+  u32 slot = 0, parity = 0;
+  auto advance = [&](u32 x) { return x + 1 == S ? 0 : x + 1; };
+  for (RowWalk rows(a, first, clusters); !rows.done(); rows.next()) {
+    const u64 r = rows.r;
+    const i32 y = rows.here();
+    const RowCut<T> cut(z + r * a.m.stride, a.m.classes);
+    const RowShare<T, NT, U> share(cut, rank, blocks);
+    const u32 groups = share.groups();
+    const bool live = u32(y) < a.m.classes, stays = backward && groups <= S;
+    float c = 0.f, base = 0.f, scale = 0.f, zy = 0.f;
+    if (live) {
+      RowScalars x = policy_scalars<kPolicy>(a, r);
+      x.zy = zy = to_f32(cut.z[y]);
+      float m = neg_inf(), s = 0.f;
+      u32 at = slot;
+      for (u32 q = 0; q < groups; ++q) {
+        copy_wait<S>(stays ? S - 1 - q : S - 1);
+        float top = m;
+        Vec<T> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (share.j0 + (q * U + u) * NT + t < share.j1) v[u].raw = ring[(at * U + u) * NT + t];
+          else v[u].fill(neg_inf());
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float f[N];
+          v[u].unpack(f);
+#pragma unroll
+          for (int k = 0; k < N; ++k) top = fmaxf(top, f[k]);
+        }
+        s = rebase(s, m, top);
+        m = top;
+        const float b = exp_base(m);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float f[N];
+          v[u].unpack(f);
+#pragma unroll
+          for (int k = 0; k < N; ++k) s += exp_fast(f[k] - b);
+        }
+        at = advance(at);
+        if (!stays) {
+          issue();
+          slot = at;
+        }
+      }
+      // the pairs of the threads, then of the warps (every warp alike), then of the blocks
+      const float wm = lanes_reduce<32>(m, MaxOp());
+      s = lanes_reduce<32>(rebase(s, m, wm), SumOp());
+      if ((t & 31) == 0) warp_part[parity][t >> 5] = make_float2(wm, s);
+      __syncthreads();
+      const float2 p = warp_part[parity][t & (kWarps - 1)];
+      m = lanes_reduce<kWarps>(p.x, MaxOp());
+      s = lanes_reduce<kWarps>(rebase(p.y, p.x, m), SumOp());
+      if (blocks > 1) cluster_join(block_part[parity], blocks, m, s);
+      parity ^= 1;  // (a row's parts are written while slower threads read the last row's)
+      base = exp_base(m);
+      scale = 1.f / s;
+      c = finish_row<kPolicy>(a, r, x, m, s, rank == 0 && t == 0);
+    } else {
+      skip_row<kPolicy>(a, r, rank == 0 && t == 0);
+    }
+    if constexpr (kPolicy) {
+      if (!backward) continue;
+      T* const g = static_cast<T*>(a.out.grad) + r * a.out.grad_stride;
+      float* const h = a.out.hess ? a.out.hess + r * a.out.hess_stride : nullptr;
+      const u32 mine = share.j0 + t;
+      if (!live) {
+        for (u32 j = mine; j < share.j1; j += NT) zero_vector(cut, j, g, h);
+        continue;
+      }
+      const float down = -c * scale;
+      for (u32 q = 0; q < groups; ++q) {
+        if (!stays) copy_wait<S>(S - 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const u32 j = mine + (q * U + u) * NT;
+          if (j < share.j1) {
+            if (c == 0.f) {
+              zero_vector(cut, j, g, h);
+            } else {
+              Vec<T> v;
+              v.raw = ring[(slot * U + u) * NT + t];
+              float f[N], e[N];
+              v.unpack(f);
+#pragma unroll
+              for (int k = 0; k < N; ++k) f[k] = exp_fast(f[k] - base);
+#pragma unroll
+              for (int k = 0; k < N; ++k) e[k] = down * f[k];
+              cut.store(g, j, e);
+              if (h) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) e[k] = margin_hess(c, f[k] * scale);
+                cut.store(h, j, e);
+              }
+            }
+          }
+        }
+        slot = advance(slot);
+        issue();
+      }
+      // the label's element, by the thread that has written its vector
+      const u32 jy = (u32(y) + cut.shift) / N;
+      if (c != 0.f && jy >= share.j0 && jy < share.j1 && (jy - share.j0) % NT == t)
+        g[y] = from_f32<T>(c * (1.f - exp_fast(zy - base) * scale));
     }
   }
 }
@@ -557,6 +680,8 @@ __global__ void __launch_bounds__(kTileRows) k_log_prob_grad_tile(GradArgs a) {
 }
 
 // ---- launches ---------------------------------------------------------------
+constexpr u32 kSMs = 148;
+constexpr int kMaxDevices = 16;
 inline u32 grid_of(u64 blocks) {
   need(blocks < (u64(1) << 31), "too many rows for one launch");
   return u32(blocks);
@@ -570,71 +695,77 @@ u32 row_vectors(const Margins& m) {
   return u32((u64(m.classes) + (even ? 0 : N - 1) + N - 1) / N);
 }
 
-template <class T, bool kPolicy, int G, int V>
-void launch_group(const RowArgs& a, u32 blocks, cudaStream_t s) {
-  if constexpr (G <= 32) {
-    k_row_loss<T, kPolicy, G, V><<<grid_of((a.m.rows + 256 / G - 1) / (256 / G)), 256, 0, s>>>(a, 1u);
-  } else {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid_of(a.m.rows * blocks));
-    cfg.blockDim = dim3(G);
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = blocks;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = blocks > 1 ? 1 : 0;
-    DP_CUDA((cudaLaunchKernelEx(&cfg, k_row_loss<T, kPolicy, G, V>, a, blocks)));
-  }
-}
 template <class T, bool kPolicy, int G>
-void launch_group_vectors(const RowArgs& a, u32 per_thread, u32 blocks, cudaStream_t s) {
-  if (per_thread <= 1) launch_group<T, kPolicy, G, 1>(a, blocks, s);
-  else if (per_thread <= 2) launch_group<T, kPolicy, G, 2>(a, blocks, s);
-  else if (per_thread <= 3) launch_group<T, kPolicy, G, 3>(a, blocks, s);
-  else if (per_thread <= 4) launch_group<T, kPolicy, G, 4>(a, blocks, s);
-  else if (per_thread <= 6) launch_group<T, kPolicy, G, 6>(a, blocks, s);
-  else launch_group<T, kPolicy, G, 8>(a, blocks, s);
+void launch_lanes(const RowArgs& a, u32 per_lane, cudaStream_t s) {
+  const u32 grid = grid_of((a.m.rows + 256 / G - 1) / (256 / G));
+  if (per_lane <= 1) k_row_loss<T, kPolicy, G, 1><<<grid, 256, 0, s>>>(a);
+  else if (per_lane <= 2) k_row_loss<T, kPolicy, G, 2><<<grid, 256, 0, s>>>(a);
+  else if (per_lane <= 3) k_row_loss<T, kPolicy, G, 3><<<grid, 256, 0, s>>>(a);
+  else if (per_lane <= 4) k_row_loss<T, kPolicy, G, 4><<<grid, 256, 0, s>>>(a);
+  else if (per_lane <= 6) k_row_loss<T, kPolicy, G, 6><<<grid, 256, 0, s>>>(a);
+  else k_row_loss<T, kPolicy, G, 8><<<grid, 256, 0, s>>>(a);
+}
+
+template <class T, bool kPolicy, int NT, int U, int S, int kPerSM>
+void launch_ring(const RowArgs& a, u32 blocks, cudaStream_t s) {
+  constexpr u32 kShared = u32(NT) * U * S * 16;
+  static_assert(kShared * kPerSM <= 220 * 1024, "the rings of an SM's blocks exceed its shared memory");
+  auto* const kernel = k_row_loss_ring<T, kPolicy, NT, U, S>;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = kShared;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = blocks > 1 ? 1 : 0;
+  // one cluster for every place that the device has for one (clusters do not
+  // fill it evenly), asked for once a device and cluster size
+  static std::atomic<int> places[kMaxDevices][kMaxCluster + 1];
+  int dev = 0;
+  DP_CUDA(cudaGetDevice(&dev));
+  int fit = dev < kMaxDevices ? places[dev][blocks].load(std::memory_order_relaxed) : 0;
+  if (fit == 0) {
+    DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kShared)));
+    if (blocks > 1) {
+      DP_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
+    } else {
+      DP_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, NT, kShared));
+      fit *= int(kSMs);
+    }
+    need(fit > 0, "the device has no place for a row's blocks");
+    if (dev < kMaxDevices) places[dev][blocks].store(fit, std::memory_order_relaxed);
+  }
+  const u32 clusters = u32(a.m.rows < u64(fit) ? a.m.rows : u64(fit));
+  cfg.gridDim = dim3(clusters * blocks);
+  DP_CUDA((cudaLaunchKernelEx(&cfg, kernel, a, blocks, clusters)));
 }
 
 template <class T, bool kPolicy>
 void launch_rows_of(const RowArgs& a, cudaStream_t s) {
   if (!a.m.rows) return;
-  constexpr u32 V = 8;  // most vectors a thread holds
+  constexpr u32 V = 8;  // most vectors a lane holds
   const u32 K = a.m.classes, nvec = row_vectors<T>(a.m);
   if (K <= kTileClasses) {
     const size_t shared = size_t(kTileRows) * (K | 1u) * sizeof(float);
     k_row_loss_tile<T, kPolicy><<<grid_of((a.m.rows + kTileRows - 1) / kTileRows), kTileRows, shared, s>>>(a);
   } else if (nvec <= 8 * V) {
-    launch_group_vectors<T, kPolicy, 8>(a, (nvec + 7) / 8, 1, s);
+    launch_lanes<T, kPolicy, 8>(a, (nvec + 7) / 8, s);
   } else if (nvec <= 32 * V) {
-    launch_group_vectors<T, kPolicy, 32>(a, (nvec + 31) / 32, 1, s);
+    launch_lanes<T, kPolicy, 32>(a, (nvec + 31) / 32, s);
+  } else if (nvec <= 1536 && a.m.rows >= 2 * kSMs) {
+    launch_ring<T, kPolicy, 128, 2, 6, 8>(a, 1, s);
   } else {
-    // a row over as few blocks as hold it, or, with few rows, over more of
-    // them so that the device is filled
-    const bool wide = nvec > kMaxCluster * 256 * V;
-    const u32 G = wide ? 512 : 256;
+    // a row over as few blocks as keep most of it in their rings, or, with
+    // few rows, over more of them so that the device is filled
     u32 blocks = 1;
-    while (blocks < kMaxCluster && (nvec > blocks * G * V || (a.m.rows * blocks < 148 && nvec > blocks * G))) blocks *= 2;
-    const u32 per = (nvec + blocks - 1) / blocks, per_thread = (per + G - 1) / G;
-    if (per_thread > V) {
-      cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3(grid_of(a.m.rows * kMaxCluster));
-      cfg.blockDim = dim3(512);
-      cfg.stream = s;
-      cudaLaunchAttribute attr{};
-      attr.id = cudaLaunchAttributeClusterDimension;
-      attr.val.clusterDim.x = kMaxCluster;
-      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-      cfg.attrs = &attr;
-      cfg.numAttrs = 1;
-      DP_CUDA((cudaLaunchKernelEx(&cfg, k_row_loss_long<T, kPolicy>, a, kMaxCluster)));
-    } else if (wide) {
-      launch_group<T, kPolicy, 512, 8>(a, blocks, s);
-    } else {
-      launch_group_vectors<T, kPolicy, 256>(a, per_thread, blocks, s);
-    }
+    while (blocks < kMaxCluster &&
+           ((kPolicy && nvec > blocks * 4096u) || (a.m.rows * blocks * 2 <= kSMs && nvec > blocks * 512u)))
+      blocks *= 2;
+    launch_ring<T, kPolicy, 512, 2, 6, 2>(a, blocks, s);
   }
   after_launch("row loss");
 }
