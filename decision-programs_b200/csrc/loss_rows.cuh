@@ -1,15 +1,16 @@
 // Row kernels of the choice losses (included by one source file a margin type).
 //
-// A row of K margins is read once and kept in registers: maximum, sum of
-// exponentials and gradient are all taken from there, so that the traffic is
-// the margins in and the gradient out, which bounds these kernels (a gradient
-// element costs two exponentials and about ten instructions for the two to
-// four bytes in and out that it moves).
+// The traffic is the margins in and the gradient out; a gradient element also
+// costs two exponentials (one for the sum, one for itself: a kept one would
+// take the room of two margins), which at 16 a clock and SM is three quarters
+// of the time that a 16-bit margin and its gradient take to move.  Everything
+// else is kept to few instructions: fp32 arithmetic is done on pairs (add, mul
+// and fma .f32x2), maxima of 16-bit margins on packed pairs.
 //
-// Rows start at any multiple of their element size.  A row is cut on 16-byte
-// boundaries of its own address: whole 16-byte vectors are moved as such, the
-// ragged first and last ones element by element, so that nothing outside the
-// row is read or written.
+// Rows start at any multiple of their element size.  A row is cut on the
+// 16-byte boundaries of its own address: whole 16-byte vectors are moved as
+// such, the few elements before the first and after the last one by one, so
+// that nothing outside the row is read or written.
 #pragma once
 #include <atomic>
 #include <cstring>
@@ -31,101 +32,240 @@ constexpr float kLog2e = 1.4426950408889634f;
 // the type's lowest value would overflow if they were scaled first.
 __device__ __forceinline__ float exp_fast(float x) { return ex2(x * kLog2e); }
 
-// 16 bytes of margins.
+// Two fp32 numbers in a register pair.
+struct Two {
+  u64 v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two ex2(Two x) {
+  float a, b;
+  x.get(a, b);
+  return Two(ex2(a), ex2(b));
+}
+
+// 16 bytes of margins as pairs.
 template <class T>
 struct Vec {
-  static constexpr int N = 16 / int(sizeof(T));
-  uint4 raw;
-  __device__ __forceinline__ void unpack(float (&f)[N]) const {
+  static constexpr int N = 16 / int(sizeof(T)), P = N / 2;
+  static __device__ __forceinline__ void unpack(const uint4& raw, Two (&f)[P]) {
     const u32 w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (sizeof(T) == 4) {
+      f[0] = Two(__uint_as_float(w[0]), __uint_as_float(w[1]));
+      f[1] = Two(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        f[i] = __uint_as_float(w[i]);
-      } else if constexpr (std::is_same<T, __half>::value) {
-        __half2 h;
-        memcpy(&h, &w[i], 4);
-        const float2 v = __half22float2(h);
-        f[2 * i] = v.x;
-        f[2 * i + 1] = v.y;
-      } else {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          __half2 h;
+          memcpy(&h, &w[i], 4);
+          const float2 v = __half22float2(h);
+          f[i] = Two(v.x, v.y);
+        } else {
+          f[i] = Two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        }
       }
     }
   }
-  __device__ __forceinline__ void pack(const float (&f)[N]) {
+  static __device__ __forceinline__ uint4 pack(const Two (&f)[P]) {
     u32 w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < P; ++i) {
+      float a, b;
+      f[i].get(a, b);
       if constexpr (sizeof(T) == 4) {
-        w[i] = __float_as_uint(f[i]);
+        w[2 * i] = __float_as_uint(a);
+        w[2 * i + 1] = __float_as_uint(b);
       } else if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        const __half2 h = __floats2half2_rn(a, b);
         memcpy(&w[i], &h, 4);
       } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         memcpy(&w[i], &h, 4);
       }
     }
-    raw = make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ __forceinline__ void fill(float v) {
-    float f[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = v;
-    pack(f);
+  // A vector of -inf, which changes no maximum and no sum.
+  static __device__ __forceinline__ uint4 none() {
+    const u32 w = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
+    return make_uint4(w, w, w, w);
+  }
+  // The larger of each place of two vectors (a NaN counts as nothing).
+  static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) {
+    return make_uint4(larger(a.x, b.x), larger(a.y, b.y), larger(a.z, b.z), larger(a.w, b.w));
+  }
+  static __device__ __forceinline__ u32 larger(u32 a, u32 b) {
+    if constexpr (sizeof(T) == 4) {
+      return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    } else {
+      typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type x, y;
+      memcpy(&x, &a, 4);
+      memcpy(&y, &b, 4);
+      x = __hmax2(x, y);
+      u32 r;
+      memcpy(&r, &x, 4);
+      return r;
+    }
+  }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    const u32 w = larger(larger(v.x, v.y), larger(v.z, v.w));
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w);
+    } else {
+      T lo, hi;
+      const u16 a = u16(w), b = u16(w >> 16);
+      memcpy(&lo, &a, 2);
+      memcpy(&hi, &b, 2);
+      return fmaxf(to_f32(lo), to_f32(hi));
+    }
   }
 };
 
-// A row cut into 16-byte vectors: vector j holds elements
-// [j N - shift, (j + 1) N - shift), of which those in [0, K) are the row's.
+// A row cut on 16-byte boundaries: whole vectors [j0, j1) counted from `base`,
+// and the elements [0, head) and [tail, K) outside them.
 template <class T>
 struct RowCut {
   static constexpr int N = Vec<T>::N;
   const T* z;
-  u32 K, shift;
-  __device__ RowCut(const T* row, u32 classes)
-      : z(row), K(classes), shift(u32(reinterpret_cast<std::uintptr_t>(row) & 15) / u32(sizeof(T))) {}
-  __device__ u32 vectors() const { return (K + shift + N - 1) / N; }
-  __device__ i64 first(u32 j) const { return i64(j) * N - shift; }
-  __device__ bool whole(u32 j) const { return (j > 0 || shift == 0) && u64(j + 1) * N <= u64(K) + shift; }
-  __device__ __forceinline__ Vec<T> load(u32 j, float outside) const {
-    Vec<T> v;
-    const i64 k0 = first(j);
-    if (whole(j)) {
-      v.raw = *reinterpret_cast<const uint4*>(z + k0);
-    } else {
-      float f[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = k0 + i >= 0 && k0 + i < i64(K) ? to_f32(z[k0 + i]) : outside;
-      v.pack(f);
-    }
-    return v;
+  const T* base;
+  u32 K, shift, j0, j1, head, tail;
+  __device__ __forceinline__ RowCut(const T* row, u32 classes) : z(row), K(classes) {
+    shift = u32(reinterpret_cast<std::uintptr_t>(row) & 15) / u32(sizeof(T));
+    base = row - shift;
+    j0 = shift ? 1 : 0;
+    j1 = max(j0, (K + shift) / N);
+    head = shift ? min(K, N - shift) : 0;
+    tail = min(K, j1 * N - shift);
   }
-  // N values of this row's vector j into a row of another array.
-  template <class U>
-  __device__ __forceinline__ void store(U* row, u32 j, const float (&f)[N]) const {
-    const i64 k0 = first(j);
-    U* const at = row + k0;
-    if (whole(j) && (reinterpret_cast<std::uintptr_t>(at) & 15) == 0) {
-      constexpr int M = Vec<U>::N;
+  // The row's elements outside the whole vectors, dealt to `G` threads.
+  template <int G, class F>
+  __device__ __forceinline__ void edges(u32 lane, F&& f) const {
 #pragma unroll
-      for (int b = 0; b < N / M; ++b) {
-        float part[M];
+    for (u32 e = lane; e < 2 * N; e += G) {
+      const u32 k = e < N ? e : tail + e - N;
+      if (e < N ? e < head : k < K) f(k);
+    }
+  }
+  // The place of element k among the vectors (an edge's is outside [j0, j1)).
+  __device__ __forceinline__ u32 vector_of(u32 k) const { return (k + shift) / N; }
+};
+
+// Where a row's gradient and curvature go: rows of other arrays addressed by
+// the margins' vectors; without a common 16-byte boundary, element by element.
+template <class T>
+struct RowOut {
+  static constexpr int N = Vec<T>::N, P = N / 2;
+  T* g;
+  float* h;
+  bool g16, h16;
+  __device__ __forceinline__ RowOut(const MarginGrad& o, u64 r, u32 shift)
+      : g(static_cast<T*>(o.grad) + r * o.grad_stride - shift), h(o.hess ? o.hess + r * o.hess_stride - shift : nullptr) {
+    g16 = (reinterpret_cast<std::uintptr_t>(g) & 15) == 0;
+    h16 = (reinterpret_cast<std::uintptr_t>(h) & 15) == 0;
+  }
+  __device__ __forceinline__ void store(u32 j, const uint4& v) const {
+    T* const at = g + u64(j) * N;
+    if (g16) {
+      *reinterpret_cast<uint4*>(at) = v;
+    } else {
+      T part[N];
+      memcpy(part, &v, 16);
 #pragma unroll
-        for (int i = 0; i < M; ++i) part[i] = f[b * M + i];
-        Vec<U> v;
-        v.pack(part);
-        reinterpret_cast<uint4*>(at)[b] = v.raw;
-      }
+      for (int i = 0; i < N; ++i) at[i] = part[i];
+    }
+  }
+  __device__ __forceinline__ void store_hess(u32 j, const Two (&f)[P]) const {
+    float* const at = h + u64(j) * N;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < P; ++i) f[i].get(v[2 * i], v[2 * i + 1]);
+    if (h16) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(at + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (k0 + i >= 0 && k0 + i < i64(K)) at[i] = from_f32<U>(f[i]);
+      for (int i = 0; i < N; ++i) at[i] = v[i];
     }
+  }
+  __device__ __forceinline__ void zero(u32 j) const {
+    store(j, make_uint4(0, 0, 0, 0));
+    if (h) {
+      Two f[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) f[i] = Two(0.f);
+      store_hess(j, f);
+    }
+  }
+  // An element k of the row, off the vectors.
+  __device__ __forceinline__ void put(u32 shift, u32 k, float gv, float hv) const {
+    g[u64(shift) + k] = from_f32<T>(gv);
+    if (h) h[u64(shift) + k] = hv;
   }
 };
+
+// How p_k comes from a margin: 2^((z - base) log2 e + low) * scale, c being
+// the derivative by the row's log-probability.
+struct RowCoef {
+  float c, base, low, scale;
+  __device__ __forceinline__ float p(float z) const { return ex2(fmaf(z - base, kLog2e, low)) * scale; }
+};
+template <class T>
+__device__ __forceinline__ void grad_vector(const RowOut<T>& out, u32 j, const uint4& raw, const RowCoef& q) {
+  constexpr int P = Vec<T>::P;
+  Two f[P], e[P];
+  Vec<T>::unpack(raw, f);
+#pragma unroll
+  for (int i = 0; i < P; ++i) f[i] = ex2(fma(f[i] + Two(-q.base), Two(kLog2e), Two(q.low)));
+#pragma unroll
+  for (int i = 0; i < P; ++i) e[i] = f[i] * Two(-q.c * q.scale);
+  out.store(j, Vec<T>::pack(e));
+  if (out.h) {
+    const float ac = fabsf(q.c), least = ac * 1e-16f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const Two p = f[i] * Two(q.scale);
+      float a, b;
+      (fma(p, Two(-1.f), Two(1.f)) * p * Two(2.f * ac)).get(a, b);
+      // (the comparison lets a NaN through)
+      e[i] = Two(a < least ? least : a, b < least ? least : b);
+    }
+    out.store_hess(j, e);
+  }
+}
+// Element k of the row by itself.
+template <class T>
+__device__ __forceinline__ void grad_element(const RowOut<T>& out, const RowCut<T>& cut, u32 k, i32 y, const RowCoef& q) {
+  float gv = 0.f, hv = 0.f;
+  if (q.c != 0.f) {
+    const float p = q.p(to_f32(cut.z[k]));
+    gv = margin_grad(q.c, p, k == u32(y));
+    hv = margin_hess(q.c, p);
+  }
+  out.put(cut.shift, k, gv, hv);
+}
+// The label's element once more, by the thread that has written its vector.
+template <class T>
+__device__ __forceinline__ void grad_label(const RowOut<T>& out, const RowCut<T>& cut, i32 y, float zy, const RowCoef& q) {
+  out.g[u64(cut.shift) + u32(y)] = from_f32<T>(margin_grad(q.c, q.p(zy), true));
+}
 
 template <int G, class Op>
 __device__ __forceinline__ float lanes_reduce(float v, Op op) {
@@ -139,6 +279,40 @@ struct MaxOp {
 struct SumOp {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
 };
+
+// A sum of exponentials relative to `from`, made relative to `to` >= from.  A
+// part that is masked throughout has from = -inf and the sum 0 (or NaN).
+__device__ __forceinline__ float rebase(float s, float from, float to) {
+  return from == neg_inf() ? s : s * exp_fast(from - to);
+}
+// A thread's running maximum and sum, joined with U more vectors.
+template <class T, int U>
+__device__ __forceinline__ void join_vectors(const uint4 (&v)[U], float& m, float& s) {
+  uint4 w = v[0];
+#pragma unroll
+  for (int u = 1; u < U; ++u) w = Vec<T>::larger(w, v[u]);
+  const float top = fmaxf(m, Vec<T>::largest(w));
+  s = rebase(s, m, top);
+  m = top;
+  const Two b(-exp_base(top));
+  Two sum[2] = {Two(s, 0.f), Two(0.f)};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    Two f[Vec<T>::P];
+    Vec<T>::unpack(v[u], f);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::P; ++i) sum[i & 1] = sum[i & 1] + ex2((f[i] + b) * Two(kLog2e));
+  }
+  float x, y;
+  (sum[0] + sum[1]).get(x, y);
+  s = x + y;
+}
+__device__ __forceinline__ void join_element(float z, float& m, float& s) {
+  const float top = fmaxf(m, z);
+  s = rebase(s, m, top) + exp_fast(z - exp_base(top));
+  m = top;
+}
+
 __device__ __forceinline__ u32 cluster_rank() {
   u32 r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -154,12 +328,6 @@ __device__ __forceinline__ void cluster_put(float2* at, u32 rank, float2 v) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(v.x), "f"(v.y) : "memory");
 }
 constexpr u32 kMaxCluster = 8;
-
-// A sum of exponentials relative to `from`, made relative to `to` >= from.  A
-// part that is masked throughout has from = -inf and the sum 0 (or NaN).
-__device__ __forceinline__ float rebase(float s, float from, float to) {
-  return from == neg_inf() ? s : s * exp_fast(from - to);
-}
 
 // The maximum and the sum over the blocks of a cluster, in the order of their
 // ranks: every block gets the same two numbers.
@@ -212,103 +380,53 @@ __device__ __forceinline__ void skip_row(const RowArgs& a, u64 r, bool writer) {
   else a.norm[r] = make_float2(0.f, 0.f);
 }
 
-// Gradient and curvature of one vector of margins, p = exp((z - base) - low) * scale.
-template <class T>
-__device__ __forceinline__ void grad_vector(const RowCut<T>& cut, u32 j, const Vec<T>& v, i32 y, float c, float base,
-                                            float low, float scale, T* g, float* h) {
-  constexpr int N = Vec<T>::N;
-  float p[N], e[N];
-  v.unpack(p);
-#pragma unroll
-  for (int i = 0; i < N; ++i) p[i] = exp_fast((p[i] - base) - low);
-  const float down = -c * scale;
-#pragma unroll
-  for (int i = 0; i < N; ++i) e[i] = down * p[i];
-  const i64 at = i64(y) - cut.first(j);  // the label's place in this vector, if it is there
-  if (at >= 0 && at < N) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (int(at) == i) e[i] = c * (1.f - p[i] * scale);
-  }
-  cut.store(g, j, e);
-  if (h) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = margin_hess(c, p[i] * scale);
-    cut.store(h, j, e);
-  }
-}
-template <class T>
-__device__ __forceinline__ void zero_vector(const RowCut<T>& cut, u32 j, T* g, float* h) {
-  constexpr int N = Vec<T>::N;
-  float e[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) e[i] = 0.f;
-  cut.store(g, j, e);
-  if (h) cut.store(h, j, e);
-}
-
 // G lanes of a warp a row, V vectors a lane, kept in registers.
 template <class T, bool kPolicy, int G, int V>
 __global__ void __launch_bounds__(256, 4) k_row_loss(RowArgs a) {
-  constexpr int N = Vec<T>::N;
   const u32 lane = threadIdx.x % G;
   const u64 r = u64(blockIdx.x) * (256 / G) + threadIdx.x / G;
   const bool in = r < a.m.rows;
   const i32 y = in ? a.label[r] : -1;
   const bool live = u32(y) < a.m.classes;
   const RowCut<T> cut(static_cast<const T*>(a.m.z) + (in ? r : 0) * a.m.stride, a.m.classes);
-  const u32 nvec = cut.vectors();
-  float c = 0.f, base = 0.f, scale = 0.f, m = neg_inf(), s = 0.f;
-  Vec<T> v[V];
+  const uint4* const z16 = reinterpret_cast<const uint4*>(cut.base);
+  float m = neg_inf(), s = 0.f;
+  uint4 v[V];
   RowScalars x;
   if (live) {
     x = policy_scalars<kPolicy>(a, r);
     x.zy = to_f32(cut.z[y]);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const u32 j = lane + i * G;
-      if (j < nvec) v[i] = cut.load(j, neg_inf());
-      else v[i].fill(neg_inf());
+      const u32 j = cut.j0 + lane + i * G;
+      v[i] = j < cut.j1 ? z16[j] : Vec<T>::none();
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float f[N];
-      v[i].unpack(f);
-#pragma unroll
-      for (int k = 0; k < N; ++k) m = fmaxf(m, f[k]);
-    }
+    if (cut.head || cut.tail < cut.K) cut.template edges<G>(lane, [&](u32 k) { join_element(to_f32(cut.z[k]), m, s); });
+    join_vectors<T, V>(v, m, s);
   }
-  m = lanes_reduce<G>(m, MaxOp());  // (the lanes of a warp reduce together, whatever their rows)
-  base = exp_base(m);
-  if (live) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float f[N];
-      v[i].unpack(f);
-#pragma unroll
-      for (int k = 0; k < N; ++k) s += exp_fast(f[k] - base);
-    }
-  }
-  s = lanes_reduce<G>(s, SumOp());
-  if (live) {
-    c = finish_row<kPolicy>(a, r, x, m, s, lane == 0);
-    scale = 1.f / s;
-  } else if (in) {
-    skip_row<kPolicy>(a, r, lane == 0);
-  }
+  const float top = lanes_reduce<G>(m, MaxOp());  // (the lanes of a warp reduce together, whatever their rows)
+  s = lanes_reduce<G>(rebase(s, m, top), SumOp());
+  float c = 0.f;
+  if (live) c = finish_row<kPolicy>(a, r, x, top, s, lane == 0);
+  else if (in) skip_row<kPolicy>(a, r, lane == 0);
   __syncwarp();  // (a gradient in the margins' place: every lane has read its label's margin)
   if constexpr (kPolicy) {
     if (!a.out.grad || !in) return;
-    T* const g = static_cast<T*>(a.out.grad) + r * a.out.grad_stride;
-    float* const h = a.out.hess ? a.out.hess + r * a.out.hess_stride : nullptr;
-    if (c == 0.f) {
-      for (u32 j = lane; j < nvec; j += G) zero_vector(cut, j, g, h);
-      return;
-    }
+    const RowOut<T> out(a.out, r, cut.shift);
+    const RowCoef q{c, exp_base(top), 0.f, 1.f / s};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const u32 j = lane + i * G;
-      if (j < nvec) grad_vector(cut, j, v[i], y, c, base, 0.f, scale, g, h);
+      const u32 j = cut.j0 + lane + i * G;
+      if (j < cut.j1) {
+        if (c == 0.f) out.zero(j);
+        else grad_vector(out, j, v[i], q);
+      }
+    }
+    if (cut.head || cut.tail < cut.K)
+      cut.template edges<G>(lane, [&](u32 k) { grad_element(out, cut, k, y, q); });
+    if (c != 0.f) {
+      const u32 jy = cut.vector_of(u32(y));
+      if (jy >= cut.j0 && jy < cut.j1 && (jy - cut.j0) % G == lane) grad_label(out, cut, y, x.zy, q);
     }
   }
 }
@@ -322,9 +440,8 @@ __global__ void __launch_bounds__(256, 4) k_row_loss(RowArgs a) {
 // so it needs no barrier.  A row that fits in the ring stays there between
 // its sum and its gradient (one read of the margins); a longer one is
 // streamed twice.
-__device__ __forceinline__ void copy_async(void* shared, const void* global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(u32(__cvta_generic_to_shared(shared))), "l"(global)
-               : "memory");
+__device__ __forceinline__ void copy_async(u32 shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most n (below S) of this thread's latest groups are under way.
@@ -342,12 +459,12 @@ __device__ __forceinline__ void copy_wait(u32 n) {
 struct RowWalk {
   const i32* label;
   u64 rows, step, r;
-  u32 classes, at = 32;
+  u32 at = 32;
   i32 batch = -1;
-  __device__ RowWalk(const RowArgs& a, u64 first, u64 clusters)
-      : label(a.label), rows(a.m.rows), step(clusters), r(first), classes(a.m.classes) {}
-  __device__ bool done() const { return r >= rows; }
-  __device__ i32 here() {
+  __device__ __forceinline__ RowWalk(const RowArgs& a, u64 first, u64 clusters)
+      : label(a.label), rows(a.m.rows), step(clusters), r(first) {}
+  __device__ __forceinline__ bool done() const { return r >= rows; }
+  __device__ __forceinline__ i32 here() {
     if (at == 32) {
       const u64 mine = r + (threadIdx.x & 31) * step;
       batch = mine < rows ? label[mine] : -1;
@@ -355,33 +472,34 @@ struct RowWalk {
     }
     return __shfl_sync(0xffffffffu, batch, at);
   }
-  __device__ void next() {
+  __device__ __forceinline__ void next() {
     r += step;
     ++at;
   }
 };
 
-// One block's share [j0, j1) of a row's vectors, in groups of NT * U.
+// One block's share [j0, j1) of a row's whole vectors, in groups of NT * U.
 template <class T, int NT, int U>
 struct RowShare {
   u32 j0 = 0, j1 = 0;
   RowShare() = default;
-  __device__ RowShare(const RowCut<T>& cut, u32 rank, u32 blocks) {
-    const u32 nvec = cut.vectors(), per = (nvec + blocks - 1) / blocks;
-    j0 = min(nvec, rank * per);
-    j1 = min(nvec, j0 + per);
+  __device__ __forceinline__ RowShare(const RowCut<T>& cut, u32 rank, u32 blocks) {
+    const u32 n = cut.j1 - cut.j0, per = blocks > 1 ? (n + blocks - 1) / blocks : n;
+    j0 = cut.j0 + min(n, rank * per);
+    j1 = min(cut.j1, j0 + per);
   }
-  __device__ u32 groups() const { return (j1 - j0 + NT * U - 1) / (NT * U); }
+  __device__ __forceinline__ u32 groups() const { return (j1 - j0 + NT * U - 1) / (NT * U); }
 };
 
 template <class T, bool kPolicy, int NT, int U, int S>
 __global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32 clusters) {
-  constexpr int N = Vec<T>::N, kWarps = NT / 32;
+  constexpr int kWarps = NT / 32;
   extern __shared__ uint4 ring[];  // [S][U][NT]
   __shared__ float2 warp_part[2][kWarps];
   __shared__ float2 block_part[2][kMaxCluster];
+  __shared__ float row_c[2];
   const u32 t = threadIdx.x, rank = blocks > 1 ? cluster_rank() : 0;
-  const u64 first = blockIdx.x / blocks;
+  const u64 first = blocks > 1 ? blockIdx.x / blocks : blockIdx.x;
   const T* const z = static_cast<const T*>(a.m.z);
   if (blocks > 1) {  // every block runs before another one writes to its memory
     cluster_arrive();
@@ -389,47 +507,52 @@ __global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32
   }
   const bool backward = kPolicy && a.out.grad != nullptr;
 
-  // the copies' place: row, share, next group, and which pass over the row
+  // the copies' place: row, next vectors, groups left, and whether the row
+  // comes once more
   RowWalk in_rows(a, first, clusters);
-  RowCut<T> in_cut(z, a.m.classes);
   RowShare<T, NT, U> in_share;
-  u32 in_group = 0, in_groups = 0, in_slot = 0;
+  const uint4* in_base = nullptr;
+  const u32 ring_at = u32(__cvta_generic_to_shared(ring + t));
+  u32 in_j = 0, in_left = 0, in_slot = 0;
   bool again = false;
   auto issue = [&]() {
-    while (in_group == in_groups && !(in_groups && again) && !in_rows.done()) {
-      const bool live = u32(in_rows.here()) < a.m.classes;
-      if (live) {
-        in_cut = RowCut<T>(z + in_rows.r * a.m.stride, a.m.classes);
-        in_share = RowShare<T, NT, U>(in_cut, rank, blocks);
-        in_group = 0;
-        in_groups = in_share.groups();
-        again = backward && in_groups > S;
+    if (in_left == 0 && again) {
+      again = false;
+      in_j = in_share.j0 + t;
+      in_left = in_share.groups();
+    }
+    while (in_left == 0 && !in_rows.done()) {
+      if (u32(in_rows.here()) < a.m.classes) {
+        const RowCut<T> cut(z + in_rows.r * a.m.stride, a.m.classes);
+        in_base = reinterpret_cast<const uint4*>(cut.base);
+        in_share = RowShare<T, NT, U>(cut, rank, blocks);
+        in_j = in_share.j0 + t;
+        in_left = in_share.groups();
+        again = backward && in_left > S;
       }
       in_rows.next();
     }
-    if (in_group == in_groups && again) {  // the second pass over a row that the ring does not hold
-      in_group = 0;
-      again = false;
-    }
-    if (in_group < in_groups) {
+    if (in_left) {
+      const uint4* const from = in_base + in_j;
+      const u32 to = ring_at + in_slot * (U * NT * 16);
+      if (in_left > 1) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const u32 j = in_share.j0 + (in_group * U + u) * NT + t;
-        uint4* const at = ring + (in_slot * U + u) * NT + t;
-        if (j < in_share.j1) {
-          if (in_cut.whole(j)) copy_async(at, in_cut.z + in_cut.first(j));
-          else *at = in_cut.load(j, neg_inf()).raw;
-        }
+        for (int u = 0; u < U; ++u) copy_async(to + u * (NT * 16), from + u * NT);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (in_j + u * NT < in_share.j1) copy_async(to + u * (NT * 16), from + u * NT);
       }
-      ++in_group;
+      in_j += U * NT;
+      --in_left;
     }
     copy_commit();  // (empty groups too: the count of groups under way stays S)
     in_slot = in_slot + 1 == S ? 0 : in_slot + 1;
   };
+#pragma unroll 1
   for (int i = 0; i < S; ++i) issue();
 
   u32 slot = 0, parity = 0;
-  auto advance = [&](u32 x) { return x + 1 == S ? 0 : x + 1; };
   for (RowWalk rows(a, first, clusters); !rows.done(); rows.next()) {
     const u64 r = rows.r;
     const i32 y = rows.here();
@@ -437,39 +560,34 @@ __global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32
     const RowShare<T, NT, U> share(cut, rank, blocks);
     const u32 groups = share.groups();
     const bool live = u32(y) < a.m.classes, stays = backward && groups <= S;
-    float c = 0.f, base = 0.f, scale = 0.f, zy = 0.f;
+    const bool ragged = rank == 0 && (cut.head || cut.tail < cut.K);
+    RowCoef q{0.f, 0.f, 0.f, 0.f};
+    float zy = 0.f;
     if (live) {
-      RowScalars x = policy_scalars<kPolicy>(a, r);
-      x.zy = zy = to_f32(cut.z[y]);
+      RowScalars x;
+      zy = to_f32(cut.z[y]);
+      if (t < 32) {
+        x = policy_scalars<kPolicy>(a, r);
+        x.zy = zy;
+      }
       float m = neg_inf(), s = 0.f;
+      if (ragged) cut.template edges<NT>(t, [&](u32 k) { join_element(to_f32(cut.z[k]), m, s); });
       u32 at = slot;
-      for (u32 q = 0; q < groups; ++q) {
-        copy_wait<S>(stays ? S - 1 - q : S - 1);
-        float top = m;
-        Vec<T> v[U];
+#pragma unroll 1
+      for (u32 i = 0; i < groups; ++i) {
+        copy_wait<S>(stays ? S - 1 - i : S - 1);
+        const uint4* const from = ring + at * (U * NT) + t;
+        uint4 v[U];
+        if (i + 1 < groups) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (share.j0 + (q * U + u) * NT + t < share.j1) v[u].raw = ring[(at * U + u) * NT + t];
-          else v[u].fill(neg_inf());
+          for (int u = 0; u < U; ++u) v[u] = from[u * NT];
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            v[u] = share.j0 + (i * U + u) * NT + t < share.j1 ? from[u * NT] : Vec<T>::none();
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float f[N];
-          v[u].unpack(f);
-#pragma unroll
-          for (int k = 0; k < N; ++k) top = fmaxf(top, f[k]);
-        }
-        s = rebase(s, m, top);
-        m = top;
-        const float b = exp_base(m);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float f[N];
-          v[u].unpack(f);
-#pragma unroll
-          for (int k = 0; k < N; ++k) s += exp_fast(f[k] - b);
-        }
-        at = advance(at);
+        join_vectors<T, U>(v, m, s);
+        at = at + 1 == S ? 0 : at + 1;
         if (!stays) {
           issue();
           slot = at;
@@ -478,62 +596,65 @@ __global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32
       // the pairs of the threads, then of the warps (every warp alike), then of the blocks
       const float wm = lanes_reduce<32>(m, MaxOp());
       s = lanes_reduce<32>(rebase(s, m, wm), SumOp());
-      if ((t & 31) == 0) warp_part[parity][t >> 5] = make_float2(wm, s);
-      __syncthreads();
-      const float2 p = warp_part[parity][t & (kWarps - 1)];
-      m = lanes_reduce<kWarps>(p.x, MaxOp());
-      s = lanes_reduce<kWarps>(rebase(p.y, p.x, m), SumOp());
+      m = wm;
+      if constexpr (kWarps > 1) {
+        if ((t & 31) == 0) warp_part[parity][t >> 5] = make_float2(m, s);
+        __syncthreads();
+        const float2 p = warp_part[parity][t & (kWarps - 1)];
+        m = lanes_reduce<kWarps>(p.x, MaxOp());
+        s = lanes_reduce<kWarps>(rebase(p.y, p.x, m), SumOp());
+      }
       if (blocks > 1) cluster_join(block_part[parity], blocks, m, s);
+      // the loss and its derivative are one warp's work
+      if (t < 32) {
+        q.c = finish_row<kPolicy>(a, r, x, m, s, rank == 0 && t == 0);
+        if (kWarps > 1 && t == 0) row_c[parity] = q.c;
+      }
+      if (kWarps > 1 && backward) {
+        __syncthreads();
+        q.c = row_c[parity];
+      }
       parity ^= 1;  // (a row's parts are written while slower threads read the last row's)
-      base = exp_base(m);
-      scale = 1.f / s;
-      c = finish_row<kPolicy>(a, r, x, m, s, rank == 0 && t == 0);
+      q.base = exp_base(m);
+      q.scale = __frcp_rn(s);
     } else {
       skip_row<kPolicy>(a, r, rank == 0 && t == 0);
     }
     if constexpr (kPolicy) {
       if (!backward) continue;
-      T* const g = static_cast<T*>(a.out.grad) + r * a.out.grad_stride;
-      float* const h = a.out.hess ? a.out.hess + r * a.out.hess_stride : nullptr;
-      const u32 mine = share.j0 + t;
-      if (!live) {
-        for (u32 j = mine; j < share.j1; j += NT) zero_vector(cut, j, g, h);
-        continue;
-      }
-      const float down = -c * scale;
-      for (u32 q = 0; q < groups; ++q) {
-        if (!stays) copy_wait<S>(S - 1);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const u32 j = mine + (q * U + u) * NT;
-          if (j < share.j1) {
-            if (c == 0.f) {
-              zero_vector(cut, j, g, h);
-            } else {
-              Vec<T> v;
-              v.raw = ring[(slot * U + u) * NT + t];
-              float f[N], e[N];
-              v.unpack(f);
-#pragma unroll
-              for (int k = 0; k < N; ++k) f[k] = exp_fast(f[k] - base);
-#pragma unroll
-              for (int k = 0; k < N; ++k) e[k] = down * f[k];
-              cut.store(g, j, e);
-              if (h) {
-#pragma unroll
-                for (int k = 0; k < N; ++k) e[k] = margin_hess(c, f[k] * scale);
-                cut.store(h, j, e);
-              }
-            }
+      if constexpr (kWarps == 1) __syncwarp();  // (in place: the label's margin has been read)
+      const RowOut<T> out(a.out, r, cut.shift);
+      if (ragged) cut.template edges<NT>(t, [&](u32 k) { grad_element(out, cut, k, y, q); });
+      if (q.c == 0.f) {
+        for (u32 j = share.j0 + t; j < share.j1; j += NT) out.zero(j);
+        if (live) {
+          for (u32 i = 0; i < groups; ++i) {
+            if (!stays) copy_wait<S>(S - 1);
+            issue();
+            slot = slot + 1 == S ? 0 : slot + 1;
           }
         }
-        slot = advance(slot);
-        issue();
+        continue;
       }
-      // the label's element, by the thread that has written its vector
-      const u32 jy = (u32(y) + cut.shift) / N;
-      if (c != 0.f && jy >= share.j0 && jy < share.j1 && (jy - share.j0) % NT == t)
-        g[y] = from_f32<T>(c * (1.f - exp_fast(zy - base) * scale));
+      u32 j = share.j0 + t;
+#pragma unroll 1
+      for (u32 i = 0; i < groups; ++i) {
+        if (!stays) copy_wait<S>(S - 1);
+        const uint4* const from = ring + slot * (U * NT) + t;
+        if (i + 1 < groups) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) grad_vector(out, j + u * NT, from[u * NT], q);
+        } else {
+#pragma unroll 1
+          for (int u = 0; u < U; ++u)
+            if (j + u * NT < share.j1) grad_vector(out, j + u * NT, from[u * NT], q);
+        }
+        j += U * NT;
+        issue();
+        slot = slot + 1 == S ? 0 : slot + 1;
+      }
+      const u32 jy = cut.vector_of(u32(y));
+      if (jy >= share.j0 && jy < share.j1 && (jy - share.j0) % NT == t) grad_label(out, cut, y, zy, q);
     }
   }
 }
@@ -609,38 +730,46 @@ __global__ void __launch_bounds__(kTileRows) k_row_loss_tile(RowArgs a) {
 
 // ---- the backward pass alone: the row's norm is given, so every element is
 // on its own.
+
 // The row's coefficient, 0 where the row has no label or no class.
 __device__ __forceinline__ float grad_weight(const GradArgs& a, u64 r, i32 y, float2 n) {
   return u32(y) < a.m.classes && !(n.x == neg_inf() && n.y == 0.f) ? a.weight[r] : 0.f;
 }
 
-// G threads take a piece of G * U vectors of a row.
+// G threads take a piece of G * U vectors of a row (the first one its edges too).
 template <class T, int G, int U>
 __global__ void __launch_bounds__(256) k_log_prob_grad(GradArgs a, u32 pieces) {
   const u64 id = u64(blockIdx.x) * (256 / G) + threadIdx.x / G;
-  const u64 r = id / pieces;
+  const u64 r = pieces > 1 ? id / pieces : id;
   if (r >= a.m.rows) return;
-  const u32 j0 = u32(id - r * pieces) * (G * U) + threadIdx.x % G;
+  const u32 piece = u32(id - r * pieces), lane = threadIdx.x % G;
   const i32 y = a.label[r];
   const float2 n = a.norm[r];
-  const float c = grad_weight(a, r, y, n);
+  const RowCoef q{grad_weight(a, r, y, n), n.x, -n.y * kLog2e, 1.f};
   const RowCut<T> cut(static_cast<const T*>(a.m.z) + r * a.m.stride, a.m.classes);
-  const u32 nvec = cut.vectors();
-  T* const g = static_cast<T*>(a.out.grad) + r * a.out.grad_stride;
-  float* const h = a.out.hess ? a.out.hess + r * a.out.hess_stride : nullptr;
-  if (c == 0.f) {
+  const RowOut<T> out(a.out, r, cut.shift);
+  const uint4* const z16 = reinterpret_cast<const uint4*>(cut.base);
+  const u32 j0 = cut.j0 + piece * (G * U), j = j0 + lane;
+  if (piece == 0 && (cut.head || cut.tail < cut.K))
+    cut.template edges<G>(lane, [&](u32 k) { grad_element(out, cut, k, y, q); });
+  if (q.c == 0.f) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (j0 + i * G < nvec) zero_vector(cut, j0 + i * G, g, h);
+      if (j + i * G < cut.j1) out.zero(j + i * G);
     return;
   }
-  Vec<T> v[U];
+  // (read before this thread overwrites its vector in place)
+  const u32 jy = cut.vector_of(u32(y));
+  const bool labels = jy >= j0 && jy < cut.j1 && jy < j0 + G * U && (jy - j0) % G == lane;
+  const float zy = labels ? to_f32(cut.z[y]) : 0.f;
+  uint4 v[U];
 #pragma unroll
   for (int i = 0; i < U; ++i)
-    if (j0 + i * G < nvec) v[i] = cut.load(j0 + i * G, neg_inf());
+    if (j + i * G < cut.j1) v[i] = z16[j + i * G];
 #pragma unroll
   for (int i = 0; i < U; ++i)
-    if (j0 + i * G < nvec) grad_vector(cut, j0 + i * G, v[i], y, c, n.x, n.y, 1.f, g, h);
+    if (j + i * G < cut.j1) grad_vector(out, j + i * G, v[i], q);
+  if (labels) grad_label(out, cut, y, zy, q);
 }
 
 // Few classes: a block takes kTileRows rows, adjacent threads adjacent elements.
@@ -686,13 +815,10 @@ inline u32 grid_of(u64 blocks) {
   need(blocks < (u64(1) << 31), "too many rows for one launch");
   return u32(blocks);
 }
-// Vectors of the longest row: one more than its elements fill when rows start
-// off the 16-byte boundaries.
+// Whole vectors of the longest row.
 template <class T>
 u32 row_vectors(const Margins& m) {
-  constexpr u64 N = 16 / sizeof(T);
-  const bool even = (reinterpret_cast<std::uintptr_t>(m.z) % 16 == 0) && (m.rows <= 1 || m.stride % N == 0);
-  return u32((u64(m.classes) + (even ? 0 : N - 1) + N - 1) / N);
+  return m.classes / u32(16 / sizeof(T));
 }
 
 template <class T, bool kPolicy, int G>
@@ -756,8 +882,10 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
     launch_lanes<T, kPolicy, 8>(a, (nvec + 7) / 8, s);
   } else if (nvec <= 32 * V) {
     launch_lanes<T, kPolicy, 32>(a, (nvec + 31) / 32, s);
-  } else if (nvec <= 1536 && a.m.rows >= 2 * kSMs) {
-    launch_ring<T, kPolicy, 128, 2, 6, 8>(a, 1, s);
+  } else if (nvec <= 1024 && a.m.rows >= 8 * kSMs) {
+    launch_ring<T, kPolicy, 32, 4, 8, 13>(a, 1, s);
+  } else if (nvec <= 2560 && a.m.rows >= 4 * kSMs) {
+    launch_ring<T, kPolicy, 128, 4, 6, 4>(a, 1, s);
   } else {
     // a row over as few blocks as keep most of it in their rings, or, with
     // few rows, over more of them so that the device is filled
@@ -765,7 +893,7 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
     while (blocks < kMaxCluster &&
            ((kPolicy && nvec > blocks * 4096u) || (a.m.rows * blocks * 2 <= kSMs && nvec > blocks * 512u)))
       blocks *= 2;
-    launch_ring<T, kPolicy, 512, 2, 6, 2>(a, blocks, s);
+    launch_ring<T, kPolicy, 256, 4, 6, 2>(a, blocks, s);
   }
   after_launch("row loss");
 }
