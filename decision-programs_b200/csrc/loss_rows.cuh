@@ -250,6 +250,42 @@ __device__ __forceinline__ void grad_vector(const RowOut<T>& out, u32 j, const u
     out.store_hess(j, e);
   }
 }
+// The same of U vectors D apart, of those below j1: without a curvature all are
+// computed before the first is stored, so that their exponentials overlap.
+template <class T, int U, int D>
+__device__ __forceinline__ void grad_vectors(const RowOut<T>& out, u32 j, u32 j1, uint4 (&v)[U], const RowCoef& q) {
+  if (out.h) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j + u * D < j1) grad_vector(out, j + u * D, v[u], q);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    constexpr int P = Vec<T>::P;
+    Two f[P];
+    Vec<T>::unpack(v[u], f);
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      f[i] = ex2(fma(f[i] + Two(-q.base), Two(kLog2e), Two(q.low))) * Two(-q.c * q.scale);
+    v[u] = Vec<T>::pack(f);
+  }
+  if (out.g16) {
+    uint4* const at = reinterpret_cast<uint4*>(out.g) + j;
+    if (j + (U - 1) * D < j1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) at[u * D] = v[u];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * D < j1) at[u * D] = v[u];
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j + u * D < j1) out.store(j + u * D, v[u]);
+  }
+}
 // Element k of the row by itself.
 template <class T>
 __device__ __forceinline__ void grad_element(const RowOut<T>& out, const RowCut<T>& cut, u32 k, i32 y, const RowCoef& q) {
@@ -414,12 +450,16 @@ __global__ void __launch_bounds__(256, 4) k_row_loss(RowArgs a) {
     if (!a.out.grad || !in) return;
     const RowOut<T> out(a.out, r, cut.shift);
     const RowCoef q{c, exp_base(top), 0.f, 1.f / s};
+    if (c == 0.f) {
+      for (u32 j = cut.j0 + lane; j < cut.j1; j += G) out.zero(j);
+    } else {
+      constexpr int U = V < 4 ? V : (V == 6 ? 3 : 4);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const u32 j = cut.j0 + lane + i * G;
-      if (j < cut.j1) {
-        if (c == 0.f) out.zero(j);
-        else grad_vector(out, j, v[i], q);
+      for (int i = 0; i < V; i += U) {
+        uint4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = v[i + u];
+        grad_vectors<T, U, G>(out, cut.j0 + lane + i * G, cut.j1, w, q);
       }
     }
     if (cut.head || cut.tail < cut.K)
@@ -483,16 +523,17 @@ template <class T, int NT, int U>
 struct RowShare {
   u32 j0 = 0, j1 = 0;
   RowShare() = default;
+  // (the blocks of a cluster are a power of two)
   __device__ __forceinline__ RowShare(const RowCut<T>& cut, u32 rank, u32 blocks) {
-    const u32 n = cut.j1 - cut.j0, per = blocks > 1 ? (n + blocks - 1) / blocks : n;
+    const u32 n = cut.j1 - cut.j0, per = (n + blocks - 1) >> (31 - __clz(blocks));
     j0 = cut.j0 + min(n, rank * per);
     j1 = min(cut.j1, j0 + per);
   }
   __device__ __forceinline__ u32 groups() const { return (j1 - j0 + NT * U - 1) / (NT * U); }
 };
 
-template <class T, bool kPolicy, int NT, int U, int S>
-__global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32 clusters) {
+template <class T, bool kPolicy, int NT, int U, int S, int kPerSM>
+__global__ void __launch_bounds__(NT, kPerSM) k_row_loss_ring(RowArgs a, u32 blocks, u32 clusters) {
   constexpr int kWarps = NT / 32;
   extern __shared__ uint4 ring[];  // [S][U][NT]
   __shared__ float2 warp_part[2][kWarps];
@@ -577,16 +618,19 @@ __global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32
       for (u32 i = 0; i < groups; ++i) {
         copy_wait<S>(stays ? S - 1 - i : S - 1);
         const uint4* const from = ring + at * (U * NT) + t;
-        uint4 v[U];
-        if (i + 1 < groups) {
+        const u32 left = share.j1 - share.j0 - i * (U * NT);
+        if (left >= U * NT) {
+          uint4 v[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) v[u] = from[u * NT];
-        } else {
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-            v[u] = share.j0 + (i * U + u) * NT + t < share.j1 ? from[u * NT] : Vec<T>::none();
+          join_vectors<T, U>(v, m, s);
+        } else {  // the last, short group: only as many vectors as there are
+#pragma unroll 1
+          for (u32 k = t; k - t < left; k += NT) {
+            const uint4 v[1] = {k < left ? from[k - t] : Vec<T>::none()};
+            join_vectors<T, 1>(v, m, s);
+          }
         }
-        join_vectors<T, U>(v, m, s);
         at = at + 1 == S ? 0 : at + 1;
         if (!stays) {
           issue();
@@ -641,13 +685,17 @@ __global__ void __launch_bounds__(NT) k_row_loss_ring(RowArgs a, u32 blocks, u32
       for (u32 i = 0; i < groups; ++i) {
         if (!stays) copy_wait<S>(S - 1);
         const uint4* const from = ring + slot * (U * NT) + t;
-        if (i + 1 < groups) {
+        if (share.j1 - (j - t) >= U * NT) {
+          uint4 v[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) grad_vector(out, j + u * NT, from[u * NT], q);
+          for (int u = 0; u < U; ++u) v[u] = from[u * NT];
+          grad_vectors<T, U, NT>(out, j, share.j1, v, q);
         } else {
 #pragma unroll 1
-          for (int u = 0; u < U; ++u)
-            if (j + u * NT < share.j1) grad_vector(out, j + u * NT, from[u * NT], q);
+          for (u32 k = j; k < share.j1; k += NT) {
+            uint4 v[1] = {from[k - j]};
+            grad_vectors<T, 1, NT>(out, k, share.j1, v, q);
+          }
         }
         j += U * NT;
         issue();
@@ -766,9 +814,7 @@ __global__ void __launch_bounds__(256) k_log_prob_grad(GradArgs a, u32 pieces) {
 #pragma unroll
   for (int i = 0; i < U; ++i)
     if (j + i * G < cut.j1) v[i] = z16[j + i * G];
-#pragma unroll
-  for (int i = 0; i < U; ++i)
-    if (j + i * G < cut.j1) grad_vector(out, j + i * G, v[i], q);
+  grad_vectors<T, U, G>(out, j, cut.j1, v, q);
   if (labels) grad_label(out, cut, y, zy, q);
 }
 
@@ -836,7 +882,7 @@ template <class T, bool kPolicy, int NT, int U, int S, int kPerSM>
 void launch_ring(const RowArgs& a, u32 blocks, cudaStream_t s) {
   constexpr u32 kShared = u32(NT) * U * S * 16;
   static_assert(kShared * kPerSM <= 220 * 1024, "the rings of an SM's blocks exceed its shared memory");
-  auto* const kernel = k_row_loss_ring<T, kPolicy, NT, U, S>;
+  auto* const kernel = k_row_loss_ring<T, kPolicy, NT, U, S, kPerSM>;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(NT);
@@ -870,6 +916,13 @@ void launch_ring(const RowArgs& a, u32 blocks, cudaStream_t s) {
   DP_CUDA((cudaLaunchKernelEx(&cfg, kernel, a, blocks, clusters)));
 }
 
+// Blocks of 256 threads a row, at least `blocks`: with few rows, as many as
+// the device has room for and the row gives each of them two vectors a thread.
+inline u32 few_rows_cluster(u64 rows, u32 nvec, u32 blocks) {
+  while (blocks < kMaxCluster && rows * blocks * 2 <= kSMs && nvec > blocks * 512u) blocks *= 2;
+  return blocks;
+}
+
 template <class T, bool kPolicy>
 void launch_rows_of(const RowArgs& a, cudaStream_t s) {
   if (!a.m.rows) return;
@@ -882,18 +935,31 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
     launch_lanes<T, kPolicy, 8>(a, (nvec + 7) / 8, s);
   } else if (nvec <= 32 * V) {
     launch_lanes<T, kPolicy, 32>(a, (nvec + 31) / 32, s);
-  } else if (nvec <= 1024 && a.m.rows >= 8 * kSMs) {
-    launch_ring<T, kPolicy, 32, 4, 8, 13>(a, 1, s);
-  } else if (nvec <= 2560 && a.m.rows >= 4 * kSMs) {
-    launch_ring<T, kPolicy, 128, 4, 6, 4>(a, 1, s);
+  } else if (!kPolicy) {
+    // Streaming: the fewer threads a row has, the less of the time goes into
+    // joining their sums, as long as the rows fill the device (134M bf16
+    // margins in rows of 8192: 46 us by 32 threads, 50 by 64, 57 by 256; of
+    // 131072, 1024 rows: 47 by 256 threads).
+    const u64 per_sm = a.m.rows / kSMs;
+    if (per_sm >= 24) launch_ring<T, kPolicy, 32, 4, 4, 24>(a, 1, s);
+    else if (per_sm >= 12) launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s);
+    else if (per_sm >= 6) launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s);
+    else launch_ring<T, kPolicy, 256, 4, 4, 3>(a, few_rows_cluster(a.m.rows, nvec, 1), s);
   } else {
-    // a row over as few blocks as keep most of it in their rings, or, with
-    // few rows, over more of them so that the device is filled
-    u32 blocks = 1;
-    while (blocks < kMaxCluster &&
-           ((kPolicy && nvec > blocks * 4096u) || (a.m.rows * blocks * 2 <= kSMs && nvec > blocks * 512u)))
-      blocks *= 2;
-    launch_ring<T, kPolicy, 256, 4, 6, 2>(a, blocks, s);
+    // As few threads as have the ring for a row, on the same grounds; a row
+    // past the largest ring is cut over a cluster of blocks.
+    const u64 per_sm = a.m.rows / kSMs;
+    if (nvec <= 512 && per_sm >= 12) {
+      launch_ring<T, kPolicy, 32, 4, 4, 24>(a, 1, s);
+    } else if (nvec <= 1024 && per_sm >= 6) {
+      launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s);
+    } else if (nvec <= 2048 && per_sm >= 3) {
+      launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s);
+    } else {
+      u32 blocks = 1;
+      while (blocks < kMaxCluster && nvec > blocks * (256u * 4 * 4)) blocks *= 2;
+      launch_ring<T, kPolicy, 256, 4, 4, 3>(a, few_rows_cluster(a.m.rows, nvec, blocks), s);
+    }
   }
   after_launch("row loss");
 }
