@@ -4,9 +4,8 @@
 // x = beta ((S_a - S_b) - (T_a - T_b)) with S, T an item's sums of scores and
 // reference scores in fp32;  L = w ((1 - e) softplus(-x) + e softplus(x)).
 // Sums run in an order that depends on the sizes alone, so that results do
-// not change from run to run.
+// not change from run to run: no floating-point atomics.
 #include <string>
-#include <vector>
 
 #include "kernels.h"
 #include "loss_math.cuh"
@@ -14,89 +13,435 @@
 namespace dp {
 namespace {
 
+constexpr u32 kSMs = 148;
+
 __device__ __forceinline__ float gap(const PairLoss& a, u64 r) { return a.ref ? a.score[r] - a.ref[r] : a.score[r]; }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Loss, gradient by the preferred item's score, curvature of one pair.
+struct PairResult {
+  float loss, q, h;
+};
+__device__ __forceinline__ PairResult pair_result(const PairLoss& a, float difference, float w) {
+  PairResult o{0.f, 0.f, 0.f};
+  if (w != 0.f) {
+    const PairTerms t = pair_terms(a.beta * difference, a.smoothing);
+    o.loss = w * t.loss;
+    o.q = w * (a.beta * t.slope);
+    o.h = w * (a.beta * a.beta * t.bend);
+  }
+  return o;
 }
 
-// An offset outside the rows is taken as the nearest end, so that no offset
-// leads outside the arrays.
-__device__ __forceinline__ u64 clamp_row(i64 b, u64 rows) { return b < 0 ? 0 : (u64(b) > rows ? rows : u64(b)); }
-
-// One warp a pair.
-__global__ void __launch_bounds__(256) k_preference(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
-  const u32 lane = threadIdx.x & 31;
-  const u64 warps = u64(gridDim.x) * (blockDim.x >> 5);
-  const u64 w0 = u64(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  for (u64 p = w0; p < pairs; p += warps) {
-    const u64 b0 = begin ? clamp_row(begin[2 * p], rows) : 2 * p;
-    const u64 b1 = begin ? clamp_row(begin[2 * p + 1], rows) : 2 * p + 1;
-    const u64 b2 = begin ? clamp_row(begin[2 * p + 2], rows) : 2 * p + 2;
-    float sa = 0.f, sb = 0.f;
-    for (u64 r = b0 + lane; r < b1; r += 32) sa += gap(a, r);
-    for (u64 r = b1 + lane; r < b2; r += 32) sb += gap(a, r);
-    sa = warp_sum(sa);
-    sb = warp_sum(sb);
-    const float w = a.weight ? a.weight[p] : 1.f;
-    float loss = 0.f, q = 0.f, h = 0.f;
-    if (w != 0.f) {
-      const PairTerms t = pair_terms(a.beta * (sa - sb), a.smoothing);
-      loss = w * t.loss;
-      q = w * (a.beta * t.slope);
-      h = w * (a.beta * a.beta * t.bend);
+// ---- consecutive items ------------------------------------------------------
+// Every row an item: a thread takes pairs of rows side by side.
+template <bool kWide>
+__global__ void __launch_bounds__(256) k_preference_rows(PairLoss a, u64 rows, u64 pairs) {
+  const u64 step = u64(gridDim.x) * blockDim.x, first = u64(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (u64 p = first; p < pairs; p += step) {
+    float sa, sb;
+    if constexpr (kWide) {
+      const float2 s = reinterpret_cast<const float2*>(a.score)[p];
+      const float2 t = a.ref ? reinterpret_cast<const float2*>(a.ref)[p] : make_float2(0.f, 0.f);
+      sa = a.ref ? s.x - t.x : s.x;
+      sb = a.ref ? s.y - t.y : s.y;
+    } else {
+      sa = gap(a, 2 * p);
+      sb = gap(a, 2 * p + 1);
     }
-    h = item_hess(h);
-    if (lane == 0) a.loss[p] = loss;
-    for (u64 r = b0 + lane; r < b1; r += 32) {
-      a.grad[r] = q;
-      if (a.hess) a.hess[r] = h;
-    }
-    for (u64 r = b1 + lane; r < b2; r += 32) {
-      a.grad[r] = -q;
-      if (a.hess) a.hess[r] = h;
+    const PairResult o = pair_result(a, sa - sb, a.weight ? a.weight[p] : 1.f);
+    a.loss[p] = o.loss;
+    const float h = item_hess(o.h);
+    if constexpr (kWide) {
+      reinterpret_cast<float2*>(a.grad)[p] = make_float2(o.q, -o.q);
+      if (a.hess) reinterpret_cast<float2*>(a.hess)[p] = make_float2(h, h);
+    } else {
+      a.grad[2 * p] = o.q;
+      a.grad[2 * p + 1] = -o.q;
+      if (a.hess) a.hess[2 * p] = a.hess[2 * p + 1] = h;
     }
   }
-  // rows before the first item and after the last belong to no pair
-  const u64 first = begin ? clamp_row(begin[0], rows) : 0, last = begin ? clamp_row(begin[2 * pairs], rows) : 2 * pairs;
-  const u64 n = first + (rows - last);
-  for (u64 i = u64(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += u64(gridDim.x) * blockDim.x) {
-    const u64 r = i < first ? i : last + (i - first);
+  for (u64 r = 2 * pairs + first; r < rows; r += step) {  // rows of no pair
     a.grad[r] = 0.f;
     if (a.hess) a.hess[r] = item_hess(0.f);
   }
 }
 
-// One thread a row; a pair's loss is written by its preferred row.
-__global__ void __launch_bounds__(256) k_pair_loss(PairLoss a, u64 rows, const u32* __restrict__ off,
-                                                   const PairEntry* __restrict__ entry) {
-  for (u64 r = u64(blockIdx.x) * blockDim.x + threadIdx.x; r < rows; r += u64(gridDim.x) * blockDim.x) {
-    const float mine = gap(a, r);
-    float g = 0.f, h = 0.f;
-    for (u32 i = off[r]; i < off[r + 1]; ++i) {
-      const PairEntry e = entry[i];
-      const bool lost = e.partner >> 31;
-      const float w = a.weight ? a.weight[e.pair] : 1.f;
-      float loss = 0.f;
-      if (w != 0.f) {
-        const float other = gap(a, e.partner & 0x7fffffffu);
-        const PairTerms t = pair_terms(a.beta * (lost ? other - mine : mine - other), a.smoothing);
-        const float q = w * (a.beta * t.slope);
-        loss = w * t.loss;
-        g += lost ? -q : q;
-        h += w * (a.beta * a.beta * t.bend);
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float span_sum(const PairLoss& a, u64 b, u64 e, u64 first, u64 step) {
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  u64 r = b + first;
+  for (; r + 3 * step < e; r += 4 * step) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] += gap(a, r + i * step);
+  }
+  for (; r < e; r += step) s[0] += gap(a, r);
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+__device__ __forceinline__ void span_fill(const PairLoss& a, u64 b, u64 e, u64 first, u64 step, float q, float h) {
+#pragma unroll 4
+  for (u64 r = b + first; r < e; r += step) {
+    a.grad[r] = q;
+    if (a.hess) a.hess[r] = h;
+  }
+}
+// An offset outside the rows is taken as the nearest end, so that no offset
+// leads outside the arrays.
+__device__ __forceinline__ u64 clamp_row(i64 b, u64 rows) { return b < 0 ? 0 : (u64(b) > rows ? rows : u64(b)); }
+// Rows before the first item and after the last belong to no pair.
+__device__ __forceinline__ void fill_outside(const PairLoss& a, u64 rows, const i64* begin, u64 pairs) {
+  const u64 first = clamp_row(begin[0], rows), last = clamp_row(begin[2 * pairs], rows);
+  const u64 me = u64(blockIdx.x) * blockDim.x + threadIdx.x, step = u64(gridDim.x) * blockDim.x;
+  span_fill(a, 0, first, me, step, 0.f, item_hess(0.f));
+  span_fill(a, last, rows, me, step, 0.f, item_hess(0.f));
+}
+
+// Short items: G lanes a pair.
+template <int G>
+__global__ void __launch_bounds__(256) k_preference_lanes(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
+  const u32 lane = threadIdx.x % G;
+  const u64 per_block = 256 / G, step = u64(gridDim.x) * per_block;
+  for (u64 p0 = u64(blockIdx.x) * per_block; p0 < pairs; p0 += step) {
+    const u64 p = p0 + threadIdx.x / G;
+    const bool in = p < pairs;  // (the lanes of a warp sum together)
+    const u64 b0 = in ? clamp_row(begin[2 * p], rows) : 0, b1 = in ? clamp_row(begin[2 * p + 1], rows) : 0,
+              b2 = in ? clamp_row(begin[2 * p + 2], rows) : 0;
+    const float sa = lanes_sum<G>(span_sum(a, b0, b1, lane, G)), sb = lanes_sum<G>(span_sum(a, b1, b2, lane, G));
+    if (!in) continue;
+    const PairResult o = pair_result(a, sa - sb, a.weight ? a.weight[p] : 1.f);
+    const float h = item_hess(o.h);
+    if (lane == 0) a.loss[p] = o.loss;
+    span_fill(a, b0, b1, lane, G, o.q, h);
+    span_fill(a, b1, b2, lane, G, -o.q, h);
+  }
+  fill_outside(a, rows, begin, pairs);
+}
+
+// Long items: a block, or a cluster of blocks, a pair.
+constexpr u32 kPairCluster = 8;
+__global__ void __launch_bounds__(512) k_preference_block(PairLoss a, u64 rows, const i64* begin, u64 pairs, u32 blocks) {
+  constexpr u32 kWarps = 512 / 32;
+  __shared__ float2 part[2][kWarps], blocks_part[2][kPairCluster];
+  u32 rank = 0, parity = 0;
+  if (blocks > 1) {
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  const u64 first = rank * 512 + threadIdx.x, step = u64(blocks) * 512;
+  for (u64 p = blockIdx.x / blocks; p < pairs; p += gridDim.x / blocks) {
+    const u64 b0 = clamp_row(begin[2 * p], rows), b1 = clamp_row(begin[2 * p + 1], rows),
+              b2 = clamp_row(begin[2 * p + 2], rows);
+    float2 s;
+    s.x = lanes_sum<32>(span_sum(a, b0, b1, first, step));
+    s.y = lanes_sum<32>(span_sum(a, b1, b2, first, step));
+    if ((threadIdx.x & 31) == 0) part[parity][threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = part[parity][threadIdx.x & (kWarps - 1)];
+    s.x = lanes_sum<kWarps>(s.x);
+    s.y = lanes_sum<kWarps>(s.y);
+    if (blocks > 1) {
+      if (threadIdx.x < blocks) {
+        const u32 here = u32(__cvta_generic_to_shared(&blocks_part[parity][rank]));
+        u32 there;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(threadIdx.x));
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(s.x), "f"(s.y) : "memory");
       }
-      if (!lost) a.loss[e.pair] = loss;
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+      s = make_float2(0.f, 0.f);
+      for (u32 b = 0; b < blocks; ++b) {
+        s.x += blocks_part[parity][b].x;
+        s.y += blocks_part[parity][b].y;
+      }
     }
-    a.grad[r] = g;
-    if (a.hess) a.hess[r] = item_hess(h);
+    parity ^= 1;  // (a pair's sums are written while slower threads read the last pair's)
+    const PairResult o = pair_result(a, s.x - s.y, a.weight ? a.weight[p] : 1.f);
+    const float h = item_hess(o.h);
+    if (first == 0) a.loss[p] = o.loss;
+    span_fill(a, b0, b1, first, step, o.q, h);
+    span_fill(a, b1, b2, first, step, -o.q, h);
+  }
+  fill_outside(a, rows, begin, pairs);
+}
+
+// ---- any pairs --------------------------------------------------------------
+// Three launches: every pair's terms once, in the pairs' order (two gathers of
+// scores a pair); then the terms summed by row over the list of (row, pair)
+// that the plan holds sorted by row, a warp taking kPairChunk entries whatever
+// rows they belong to, so that one row in very many pairs costs no more than
+// many rows in few; then the rows that reach over several chunks.  Bound by
+// the random 32-byte sectors of the gathers (two a pair of 4-byte scores, two
+// of 8-byte terms), which L2 serves.
+
+__global__ void __launch_bounds__(256) k_gap(const float* score, const float* ref, u64 rows, float* out) {
+  for (u64 r = u64(blockIdx.x) * blockDim.x + threadIdx.x; r < rows; r += u64(gridDim.x) * blockDim.x)
+    out[r] = score[r] - ref[r];
+}
+
+__global__ void __launch_bounds__(256) k_pair_terms(PairLoss a, const float* score, const int2* __restrict__ pair,
+                                                    u64 pairs, u64 rows, float2* terms) {
+  constexpr int U = 4;
+  const u64 step = u64(gridDim.x) * blockDim.x, first = u64(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (u64 p0 = first; p0 < pairs; p0 += U * step) {
+    float d[U], w[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const u64 p = p0 + i * step;
+      d[i] = w[i] = 0.f;
+      if (p < pairs) {
+        const int2 x = pair[p];
+        d[i] = score[x.x] - score[x.y];
+        w[i] = a.weight ? a.weight[p] : 1.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const u64 p = p0 + i * step;
+      if (p >= pairs) break;
+      const PairResult o = pair_result(a, d[i], w[i]);
+      a.loss[p] = o.loss;
+      terms[p] = make_float2(o.q, o.h);
+    }
+  }
+  for (u64 r = first; r < rows; r += step) {  // (rows of no pair keep these)
+    a.grad[r] = 0.f;
+    if (a.hess) a.hess[r] = item_hess(0.f);
   }
 }
 
-u32 blocks_for(u64 n, u64 per_block) {
-  const u64 want = (n + per_block - 1) / per_block, cap = 148 * 64;
+__device__ __forceinline__ void put_row(const PairLoss& a, u32 row, float2 s) {
+  a.grad[row] = s.x;
+  if (a.hess) a.hess[row] = item_hess(s.y);
+}
+
+// One warp a chunk of entries.  A row that begins and ends in the chunk is
+// written here; of one that began before, this chunk's sum goes to part[c].x
+// place `kHead`, of one that goes on after it to `kTail`.
+__global__ void __launch_bounds__(256) k_pair_rows(PairLoss a, const PairEntry* __restrict__ entry, u64 n,
+                                                   const float2* __restrict__ terms, float2* head, float2* tail) {
+  constexpr int kSteps = kPairChunk / 32;
+  const u32 lane = threadIdx.x & 31;
+  const u64 c = u64(blockIdx.x) * 8 + (threadIdx.x >> 5), base = c * kPairChunk;
+  if (base >= n) return;
+  constexpr u32 kNone = 0xffffffffu;  // past every row
+  u32 row[kSteps];
+  float2 v[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const u64 e = base + i * 32 + lane;
+    PairEntry x{kNone, 0};
+    if (e < n) x = entry[e];
+    row[i] = x.row;
+    v[i] = e < n ? terms[x.pair & 0x7fffffffu] : make_float2(0.f, 0.f);
+    if (x.pair >> 31) v[i].x = -v[i].x;
+  }
+  const u32 first = __shfl_sync(0xffffffffu, row[0], 0);
+  const u32 before = base ? entry[base - 1].row : kNone, after = base + kPairChunk < n ? entry[base + kPairChunk].row : kNone;
+  const bool begun = before == first;
+  u32 open = kNone;  // the row that the last step ended in, and its sum
+  float2 sum = make_float2(0.f, 0.f);
+  auto close = [&](u32 r, float2 s) {
+    if (r == kNone) return;
+    if (r == first && begun) head[c] = s;
+    else put_row(a, r, s);
+  };
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const u32 r = row[i], up = __shfl_up_sync(0xffffffffu, r, 1);
+    const u32 starts = __ballot_sync(0xffffffffu, lane == 0 ? r != open : r != up);
+    // (lane 0 of a step that goes on with the open row takes its sum in)
+    if (lane == 0) {
+      if (starts & 1) close(open, sum);
+      else v[i] = make_float2(sum.x + v[i].x, sum.y + v[i].y);
+    }
+    const u32 upto = starts & (0xffffffffu >> (31 - lane));
+    const u32 reach = upto ? lane - (31 - __clz(upto)) : lane;
+    float2 s = v[i];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const float x = __shfl_up_sync(0xffffffffu, s.x, d), y = __shfl_up_sync(0xffffffffu, s.y, d);
+      if (u32(d) <= reach) {
+        s.x += x;
+        s.y += y;
+      }
+    }
+    if (lane < 31 && (starts >> (lane + 1) & 1)) close(r, s);
+    open = __shfl_sync(0xffffffffu, r, 31);
+    sum.x = __shfl_sync(0xffffffffu, s.x, 31);
+    sum.y = __shfl_sync(0xffffffffu, s.y, 31);
+  }
+  if (lane != 0 || open == kNone) return;
+  if (open != after) close(open, sum);
+  else if (open == first && begun) head[c] = sum;  // the whole chunk is one row's
+  else tail[c] = sum;
+}
+
+// The rows that end in a chunk that they did not begin in: the tail of the
+// chunk where they began, then the heads of those since.
+__global__ void __launch_bounds__(256) k_pair_joins(PairLoss a, const PairEntry* __restrict__ entry, u64 n,
+                                                    const float2* head, const float2* tail) {
+  const u32 lane = threadIdx.x & 31;
+  const u64 c = u64(blockIdx.x) * 256 + threadIdx.x, base = c * kPairChunk;
+  u32 row = 0;
+  bool ends = false;
+  u64 from = 0;
+  if (c > 0 && base < n) {
+    const u64 end = min(n, base + u64(kPairChunk));
+    row = entry[base].row;
+    ends = entry[base - 1].row == row && (end == n || entry[end].row != row);
+    if (ends) {  // the first chunk that holds entries of the row
+      u64 lo = 0, hi = base - 1;  // entry[hi].row == row
+      if (entry[base - kPairChunk].row != row) lo = base - kPairChunk;
+      while (lo < hi) {
+        const u64 mid = (lo + hi) / 2;
+        if (entry[mid].row < row) lo = mid + 1;
+        else hi = mid;
+      }
+      from = lo / kPairChunk;
+    }
+  }
+  const bool wide = ends && c - from > 32;
+  if (ends && !wide) {
+    float2 s = tail[from];
+    for (u64 k = from + 1; k <= c; ++k) {
+      const float2 x = head[k];
+      s.x += x.x;
+      s.y += x.y;
+    }
+    put_row(a, row, s);
+  }
+  for (u32 todo = __ballot_sync(0xffffffffu, wide); todo; todo &= todo - 1) {
+    const int src = __ffs(int(todo)) - 1;
+    const u64 f = __shfl_sync(0xffffffffu, from, src), l = __shfl_sync(0xffffffffu, c, src);
+    const u32 r = __shfl_sync(0xffffffffu, row, src);
+    float2 s = make_float2(0.f, 0.f);
+    for (u64 k = f + lane; k <= l; k += 32) {
+      const float2 x = k == f ? tail[k] : head[k];
+      s.x += x.x;
+      s.y += x.y;
+    }
+    s.x = lanes_sum<32>(s.x);
+    s.y = lanes_sum<32>(s.y);
+    if (lane == 0) put_row(a, r, s);
+  }
+}
+
+// ---- the plan: (row, pair) entries sorted by row, by a least-significant-
+// digit radix sort, which keeps the pairs of a row in their order.
+__global__ void __launch_bounds__(256) k_pair_entries(const int2* __restrict__ pair, u64 pairs, u64 rows, PairEntry* out,
+                                                      unsigned long long* bad) {
+  for (u64 p = u64(blockIdx.x) * blockDim.x + threadIdx.x; p < pairs; p += u64(gridDim.x) * blockDim.x) {
+    const int2 x = pair[p];
+    const bool outside = x.x < 0 || x.y < 0 || u64(x.x) >= rows || u64(x.y) >= rows;
+    if (outside || x.x == x.y) atomicMin(bad, (unsigned long long)(2 * p + (outside ? 0 : 1)));
+    out[2 * p] = PairEntry{u32(x.x), u32(p)};
+    out[2 * p + 1] = PairEntry{u32(x.y), u32(p) | 0x80000000u};
+  }
+}
+
+constexpr int kDigitBits = 8, kDigits = 1 << kDigitBits, kSortWarps = 8, kSortSteps = 16;
+constexpr u32 kSortTile = kSortWarps * kSortSteps * 32;
+
+__device__ __forceinline__ u32 digit_of(u32 row, int shift) { return (row >> shift) & (kDigits - 1); }
+
+// Lanes of this warp with the same digit (`in`: lanes that hold an entry).
+__device__ __forceinline__ u32 same_digit(u32 digit, bool in) {
+  return __match_any_sync(0xffffffffu, in ? digit : kDigits);
+}
+
+__global__ void __launch_bounds__(256) k_sort_count(const PairEntry* __restrict__ in, u64 n, int shift, u32 blocks,
+                                                    u32* count) {
+  __shared__ u32 c[kDigits];
+  c[threadIdx.x] = 0;
+  __syncthreads();
+  const u64 base = u64(blockIdx.x) * kSortTile;
+  for (u32 i = threadIdx.x; i < kSortTile && base + i < n; i += 256) atomicAdd(&c[digit_of(in[base + i].row, shift)], 1u);
+  __syncthreads();
+  count[u64(threadIdx.x) * blocks + blockIdx.x] = c[threadIdx.x];
+}
+
+// One block a digit: its counts become exclusive sums over the tiles, and
+// total[digit] the digit's count.
+__global__ void __launch_bounds__(256) k_sort_scan(u32* count, u32 blocks, u32* total) {
+  __shared__ u32 warp[8];
+  u32* const row = count + u64(blockIdx.x) * blocks;
+  const u32 lane = threadIdx.x & 31;
+  u32 carry = 0;
+  for (u32 b0 = 0; b0 < blocks; b0 += 256) {
+    const u32 b = b0 + threadIdx.x, mine = b < blocks ? row[b] : 0;
+    u32 s = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const u32 x = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= u32(d)) s += x;
+    }
+    if (lane == 31) warp[threadIdx.x >> 5] = s;
+    __syncthreads();
+    u32 below = 0, all = 0;
+    for (u32 w = 0; w < 8; ++w) {
+      if (w < threadIdx.x >> 5) below += warp[w];
+      all += warp[w];
+    }
+    if (b < blocks) row[b] = carry + below + s - mine;
+    carry += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) total[blockIdx.x] = carry;
+}
+
+// Moves a tile's entries to their places: digit, then tile, then the order in
+// the tile (a warp holds kSortSteps * 32 consecutive entries of it).
+__global__ void __launch_bounds__(256) k_sort_move(const PairEntry* __restrict__ in, u64 n, int shift, u32 blocks,
+                                                   const u32* __restrict__ count, const u32* __restrict__ total,
+                                                   PairEntry* out) {
+  __shared__ u32 at[kSortWarps][kDigits];
+  __shared__ u32 scan[kDigits];
+  const u32 t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  for (int w = 0; w < kSortWarps; ++w) at[w][t] = 0;
+  scan[t] = total[t];
+  __syncthreads();
+  const u64 base = u64(blockIdx.x) * kSortTile + u64(warp) * kSortSteps * 32;
+  for (int i = 0; i < kSortSteps; ++i) {
+    const u64 e = base + i * 32 + lane;
+    const u32 d = e < n ? digit_of(in[e].row, shift) : 0;
+    const u32 same = same_digit(d, e < n);
+    if (e < n && (same & ((1u << lane) - 1)) == 0) at[warp][d] += __popc(same);
+    __syncwarp();
+  }
+  // inclusive sums of the digits' totals
+  for (u32 d = 1; d < kDigits; d <<= 1) {
+    const u32 x = t >= d ? scan[t - d] : 0;
+    __syncthreads();
+    scan[t] += x;
+    __syncthreads();
+  }
+  u32 place = scan[t] - total[t] + count[u64(t) * blocks + blockIdx.x];
+  for (int w = 0; w < kSortWarps; ++w) {
+    const u32 m = at[w][t];
+    at[w][t] = place;
+    place += m;
+  }
+  __syncthreads();
+  for (int i = 0; i < kSortSteps; ++i) {
+    const u64 e = base + i * 32 + lane;
+    PairEntry x{0, 0};
+    if (e < n) x = in[e];
+    const u32 d = digit_of(x.row, shift), same = same_digit(d, e < n), lower = same & ((1u << lane) - 1);
+    u32 to = 0;
+    if (e < n) to = at[warp][d] + __popc(lower);
+    __syncwarp();
+    if (e < n && lower == 0) at[warp][d] += __popc(same);
+    if (e < n) out[to] = x;
+    __syncwarp();
+  }
+}
+
+u32 blocks_for(u64 n, u64 per_block, u64 cap = u64(kSMs) * 16) {
+  const u64 want = (n + per_block - 1) / per_block;
   return u32(want < 1 ? 1 : (want < cap ? want : cap));
 }
 
@@ -104,7 +449,34 @@ u32 blocks_for(u64 n, u64 per_block) {
 
 void launch_preference(const PairLoss& a, u64 rows, const i64* begin, u64 pairs, cudaStream_t s) {
   if (!rows && !pairs) return;
-  k_preference<<<blocks_for(pairs, 8), 256, 0, s>>>(a, rows, begin, pairs);
+  const u64 average = pairs ? rows / pairs : rows;  // rows of a pair
+  if (!begin) {
+    const auto odd = [](const float* p) { return reinterpret_cast<std::uintptr_t>(p) & 7; };
+    if (odd(a.score) || odd(a.ref) || odd(a.grad) || odd(a.hess))
+      k_preference_rows<false><<<blocks_for(rows / 2 + 1, 256), 256, 0, s>>>(a, rows, pairs);
+    else
+      k_preference_rows<true><<<blocks_for(rows / 2 + 1, 256), 256, 0, s>>>(a, rows, pairs);
+  } else if (average < 64 && pairs >= 64) {
+    k_preference_lanes<8><<<blocks_for(pairs, 32), 256, 0, s>>>(a, rows, begin, pairs);
+  } else if (average < 1024 && pairs >= 4 * kSMs) {
+    k_preference_lanes<32><<<blocks_for(pairs, 8), 256, 0, s>>>(a, rows, begin, pairs);
+  } else {
+    // a block a pair; few pairs of very many rows: a cluster of blocks each
+    u32 blocks = 1;
+    while (blocks < kPairCluster && pairs * blocks * 2 <= kSMs && average > 4096u * blocks) blocks *= 2;
+    const u64 clusters = pairs < 1 ? 1 : (pairs < kSMs * 4 ? pairs : kSMs * 4);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(u32(clusters * blocks));
+    cfg.blockDim = dim3(512);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = blocks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = blocks > 1 ? 1 : 0;
+    DP_CUDA((cudaLaunchKernelEx(&cfg, k_preference_block, a, rows, begin, pairs, blocks)));
+  }
   after_launch("preference loss");
 }
 
@@ -112,38 +484,80 @@ void build_pair_plan(PairPlan& plan, u64 rows, const i32* pair_rows, u64 pairs, 
   DP_CUDA(cudaGetDevice(&plan.device));
   plan.rows = rows;
   plan.pairs = pairs;
-  std::vector<i32> list(2 * pairs);
-  if (pairs)
-    DP_CUDA(cudaMemcpyAsync(list.data(), pair_rows, list.size() * sizeof(i32), cudaMemcpyDeviceToHost, s));
+  if (!pairs) return;
+  const u64 n = 2 * pairs, chunks = (n + kPairChunk - 1) / kPairChunk;
+  SlabPlan slab;
+  slab.want(plan.pair, pairs);
+  slab.want(plan.entry, n);
+  slab.want(plan.terms, pairs);
+  slab.want(plan.head, chunks);
+  slab.want(plan.tail, chunks);
+  slab.want(plan.gap, rows);
+  slab.commit(plan.slabs, plan.device);
+  const u32 tiles = u32((n + kSortTile - 1) / kSortTile);
+  DevBuf<PairEntry> other;
+  DevBuf<u32> count, total;
+  DevBuf<unsigned long long> bad;
+  SlabPlan work;
+  work.want(other, n);
+  work.want(count, u64(kDigits) * tiles);
+  work.want(total, kDigits);
+  work.want(bad, 1);
+  std::vector<DevBuf<unsigned char>> scratch;
+  work.commit(scratch, plan.device);
+  DP_CUDA(cudaMemcpyAsync(plan.pair.get(), pair_rows, pairs * sizeof(int2), cudaMemcpyDeviceToDevice, s));
+  DP_CUDA(cudaMemsetAsync(bad.get(), 0xff, sizeof(unsigned long long), s));
+  int passes = 0;
+  while (passes * kDigitBits < 32 && (rows - 1) >> (passes * kDigitBits)) ++passes;
+  // an even number of passes ends where it began
+  PairEntry *from = passes % 2 ? other.get() : plan.entry.get(), *to = passes % 2 ? plan.entry.get() : other.get();
+  k_pair_entries<<<blocks_for(pairs, 256), 256, 0, s>>>(plan.pair.get(), pairs, rows, from, bad.get());
+  after_launch("pair entries");
+  unsigned long long worst = 0;
+  DP_CUDA(cudaMemcpyAsync(&worst, bad.get(), sizeof worst, cudaMemcpyDeviceToHost, s));
   DP_CUDA(cudaStreamSynchronize(s));
-  std::vector<u32> off(rows + 1, 0);
-  for (u64 p = 0; p < pairs; ++p) {
-    const i32 x = list[2 * p], y = list[2 * p + 1];
-    if (x < 0 || y < 0 || u64(x) >= rows || u64(y) >= rows)
-      fail("pair " + std::to_string(p) + " names a row outside [0, " + std::to_string(rows) + ")");
-    if (x == y) fail("pair " + std::to_string(p) + " names one row twice");
-    ++off[u64(x) + 1];
-    ++off[u64(y) + 1];
+  if (worst != ~0ull)
+    fail("pair " + std::to_string(worst / 2) +
+         (worst % 2 ? std::string(" names one row twice") : " names a row outside [0, " + std::to_string(rows) + ")"));
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * kDigitBits;
+    k_sort_count<<<tiles, 256, 0, s>>>(from, n, shift, tiles, count.get());
+    after_launch("pair sort");
+    k_sort_scan<<<kDigits, 256, 0, s>>>(count.get(), tiles, total.get());
+    after_launch("pair sort");
+    k_sort_move<<<tiles, 256, 0, s>>>(from, n, shift, tiles, count.get(), total.get(), to);
+    after_launch("pair sort");
+    std::swap(from, to);
   }
-  for (u64 r = 0; r < rows; ++r) off[r + 1] += off[r];
-  std::vector<PairEntry> entry(2 * pairs);
-  std::vector<u32> at(off.begin(), off.end());
-  for (u64 p = 0; p < pairs; ++p) {
-    const u32 x = u32(list[2 * p]), y = u32(list[2 * p + 1]);
-    entry[at[x]++] = PairEntry{y, u32(p)};
-    entry[at[y]++] = PairEntry{x | 0x80000000u, u32(p)};
-  }
-  plan.off.resize(rows + 1);
-  plan.entry.resize(2 * pairs);
-  DP_CUDA(cudaMemcpy(plan.off.get(), off.data(), off.size() * sizeof(u32), cudaMemcpyHostToDevice));
-  if (pairs)
-    DP_CUDA(cudaMemcpy(plan.entry.get(), entry.data(), entry.size() * sizeof(PairEntry), cudaMemcpyHostToDevice));
+  DP_CUDA(cudaStreamSynchronize(s));
+  for (auto& b : scratch) SlabCache::give(plan.device, std::move(b));
+}
+
+PairPlan::~PairPlan() {
+  if (slabs.empty()) return;
+  cudaDeviceSynchronize();  // no run of the plan is under way when its memory goes to the next one
+  for (auto& b : slabs) SlabCache::give(device, std::move(b));
 }
 
 void launch_pair_loss(const PairPlan& p, const PairLoss& a, cudaStream_t s) {
   if (!p.rows) return;
-  k_pair_loss<<<blocks_for(p.rows, 256), 256, 0, s>>>(a, p.rows, p.off.get(), p.entry.get());
+  const float* score = a.score;
+  if (a.ref && p.pairs) {
+    k_gap<<<blocks_for(p.rows, 256), 256, 0, s>>>(a.score, a.ref, p.rows, p.gap.get());
+    after_launch("pair loss");
+    score = p.gap.get();
+  }
+  const u64 most = p.pairs > p.rows ? p.pairs : p.rows;
+  k_pair_terms<<<blocks_for(most, 256), 256, 0, s>>>(a, score, p.pair.get(), p.pairs, p.rows, p.terms.get());
   after_launch("pair loss");
+  if (!p.pairs) return;
+  const u64 n = 2 * p.pairs, chunks = (n + kPairChunk - 1) / kPairChunk;
+  k_pair_rows<<<u32((chunks + 7) / 8), 256, 0, s>>>(a, p.entry.get(), n, p.terms.get(), p.head.get(), p.tail.get());
+  after_launch("pair loss");
+  if (chunks > 1) {
+    k_pair_joins<<<u32((chunks + 255) / 256), 256, 0, s>>>(a, p.entry.get(), n, p.head.get(), p.tail.get());
+    after_launch("pair loss");
+  }
 }
 
 }  // namespace dp

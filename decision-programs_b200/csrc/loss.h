@@ -82,17 +82,27 @@ struct PairLoss {
 };
 void launch_preference(const PairLoss& a, u64 rows, const i64* begin, u64 pairs, cudaStream_t s);
 
-// Any pairs over rows, laid out by row once: the pairs that row r takes part
-// in are entries [off[r], off[r + 1]) in ascending order of the pair.
+// Any pairs over rows, laid out once: a copy of the pairs, and an entry for
+// each row of each pair, sorted by row and within a row by pair; workspace of
+// a run (one at a time).
 struct PairEntry {
-  u32 partner;  // the other row; bit 31 set: r is the one not preferred
-  u32 pair;
+  u32 row;
+  u32 pair;  // bit 31 set: the row is the one not preferred
 };
+constexpr u32 kPairChunk = 256;  // entries that one warp sums
 struct PairPlan {
   u64 rows = 0, pairs = 0;
   int device = 0;
-  DevBuf<u32> off;
+  std::vector<DevBuf<unsigned char>> slabs;  // memory of the views below
+  DevBuf<int2> pair;
   DevBuf<PairEntry> entry;
+  DevBuf<float2> terms;        // [pairs] derivative by the preferred score, curvature
+  DevBuf<float2> head, tail;   // [chunks] sums of rows that reach over chunks
+  DevBuf<float> gap;           // [rows] score - ref
+  PairPlan() = default;
+  ~PairPlan();  // the plan's device is current
+  PairPlan(const PairPlan&) = delete;
+  PairPlan& operator=(const PairPlan&) = delete;
 };
 // Checks the pairs (device, [pairs][2]: preferred row, other row) and lays
 // them out; waits for `s`.  Throws when a pair names a row outside

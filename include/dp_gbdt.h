@@ -355,8 +355,9 @@ DP_API int dp_preference_loss(uint64_t rows, const int64_t* item_begin, uint64_t
  * preferred row, other row; a row may be in any number of pairs, and its
  * gradient and curvature sum over them.  dp_preference_prepare checks the
  * pairs (a row out of range or a pair of one row with itself is refused),
- * lays them out once and waits for `stream`; dp_preference_run then runs on
- * that layout, which it does not change, so runs of one plan may overlap. */
+ * copies and sorts them once and waits for `stream`; dp_preference_run then
+ * runs on that layout and the plan's workspace: order the runs of one plan
+ * (one stream, or events).  dp_preference_free waits for the device. */
 DP_API int dp_preference_prepare(uint64_t rows, const int32_t* pair_rows, uint64_t pairs, void* stream,
                                  void** out_plan);
 DP_API int dp_preference_run(void* plan, const float* score, const float* ref_score, const float* weight, float beta,
