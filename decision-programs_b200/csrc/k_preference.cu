@@ -193,9 +193,9 @@ __global__ void __launch_bounds__(256) k_pair_terms(PairLoss a, const float* sco
       const u64 p = p0 + i * step;
       d[i] = w[i] = 0.f;
       if (p < pairs) {
-        const int2 x = pair[p];
+        const int2 x = __ldcs(pair + p);
         d[i] = score[x.x] - score[x.y];
-        w[i] = a.weight ? a.weight[p] : 1.f;
+        w[i] = a.weight ? __ldcs(a.weight + p) : 1.f;
       }
     }
 #pragma unroll
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(256) k_pair_terms(PairLoss a, const float* sco
       const u64 p = p0 + i * step;
       if (p >= pairs) break;
       const PairResult o = pair_result(a, d[i], w[i]);
-      a.loss[p] = o.loss;
+      __stcs(a.loss + p, o.loss);
       terms[p] = make_float2(o.q, o.h);
     }
   }
@@ -219,35 +219,43 @@ __device__ __forceinline__ void put_row(const PairLoss& a, u32 row, float2 s) {
 }
 
 // One warp a chunk of entries.  A row that begins and ends in the chunk is
-// written here; of one that began before, this chunk's sum goes to part[c].x
-// place `kHead`, of one that goes on after it to `kTail`.
+// written here; of one that began before, this chunk's sum goes to head[c], of
+// one that goes on after it to tail[c].  joins[c]: the row that ends in the
+// chunk without having begun there, kInside where the whole chunk is part of
+// one that goes on, kNoRow where there is neither.
+constexpr u32 kNoRow = 0xffffffffu, kInside = 0xfffffffeu;  // past every row
 __global__ void __launch_bounds__(256) k_pair_rows(PairLoss a, const PairEntry* __restrict__ entry, u64 n,
-                                                   const float2* __restrict__ terms, float2* head, float2* tail) {
+                                                   const float2* __restrict__ terms, float2* head, float2* tail,
+                                                   u32* joins) {
   constexpr int kSteps = kPairChunk / 32;
   const u32 lane = threadIdx.x & 31;
   const u64 c = u64(blockIdx.x) * 8 + (threadIdx.x >> 5), base = c * kPairChunk;
   if (base >= n) return;
-  constexpr u32 kNone = 0xffffffffu;  // past every row
   u32 row[kSteps];
   float2 v[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const u64 e = base + i * 32 + lane;
-    PairEntry x{kNone, 0};
-    if (e < n) x = entry[e];
-    row[i] = x.row;
-    v[i] = e < n ? terms[x.pair & 0x7fffffffu] : make_float2(0.f, 0.f);
-    if (x.pair >> 31) v[i].x = -v[i].x;
+    uint2 x = make_uint2(kNoRow, 0);
+    if (e < n) x = __ldcs(reinterpret_cast<const uint2*>(entry) + e);  // (read once: L2 is kept for the terms)
+    row[i] = x.x;
+    v[i] = e < n ? terms[x.y & 0x7fffffffu] : make_float2(0.f, 0.f);
+    if (x.y >> 31) v[i].x = -v[i].x;
   }
   const u32 first = __shfl_sync(0xffffffffu, row[0], 0);
-  const u32 before = base ? entry[base - 1].row : kNone, after = base + kPairChunk < n ? entry[base + kPairChunk].row : kNone;
+  const u32 before = base ? entry[base - 1].row : kNoRow, after = base + kPairChunk < n ? entry[base + kPairChunk].row : kNoRow;
   const bool begun = before == first;
-  u32 open = kNone;  // the row that the last step ended in, and its sum
+  u32 open = kNoRow;  // the row that the last step ended in, and its sum
   float2 sum = make_float2(0.f, 0.f);
+  u32 join = kNoRow;
   auto close = [&](u32 r, float2 s) {
-    if (r == kNone) return;
-    if (r == first && begun) head[c] = s;
-    else put_row(a, r, s);
+    if (r == kNoRow) return;
+    if (r == first && begun) {
+      head[c] = s;
+      join = r;
+    } else {
+      put_row(a, r, s);
+    }
   };
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
@@ -274,35 +282,37 @@ __global__ void __launch_bounds__(256) k_pair_rows(PairLoss a, const PairEntry* 
     sum.x = __shfl_sync(0xffffffffu, s.x, 31);
     sum.y = __shfl_sync(0xffffffffu, s.y, 31);
   }
-  if (lane != 0 || open == kNone) return;
-  if (open != after) close(open, sum);
-  else if (open == first && begun) head[c] = sum;  // the whole chunk is one row's
-  else tail[c] = sum;
+  if (lane == 0 && open != kNoRow) {
+    if (open != after) {
+      close(open, sum);
+    } else if (open == first && begun) {  // the whole chunk is one row's
+      head[c] = sum;
+      join = kInside;
+    } else {
+      tail[c] = sum;
+    }
+  }
+  join = __reduce_min_sync(0xffffffffu, join);  // (one lane's at most)
+  if (lane == 0) joins[c] = join;
 }
 
 // The rows that end in a chunk that they did not begin in: the tail of the
 // chunk where they began, then the heads of those since.
-__global__ void __launch_bounds__(256) k_pair_joins(PairLoss a, const PairEntry* __restrict__ entry, u64 n,
-                                                    const float2* head, const float2* tail) {
+__global__ void __launch_bounds__(256) k_pair_joins(PairLoss a, const PairEntry* __restrict__ entry, u64 chunks,
+                                                    const float2* head, const float2* tail, const u32* joins) {
   const u32 lane = threadIdx.x & 31;
-  const u64 c = u64(blockIdx.x) * 256 + threadIdx.x, base = c * kPairChunk;
-  u32 row = 0;
-  bool ends = false;
-  u64 from = 0;
-  if (c > 0 && base < n) {
-    const u64 end = min(n, base + u64(kPairChunk));
-    row = entry[base].row;
-    ends = entry[base - 1].row == row && (end == n || entry[end].row != row);
-    if (ends) {  // the first chunk that holds entries of the row
-      u64 lo = 0, hi = base - 1;  // entry[hi].row == row
-      if (entry[base - kPairChunk].row != row) lo = base - kPairChunk;
-      while (lo < hi) {
-        const u64 mid = (lo + hi) / 2;
-        if (entry[mid].row < row) lo = mid + 1;
-        else hi = mid;
-      }
-      from = lo / kPairChunk;
+  const u64 c = u64(blockIdx.x) * 256 + threadIdx.x;
+  const u32 row = c < chunks ? joins[c] : kNoRow;
+  const bool ends = row < kInside;
+  u64 from = c - 1;
+  if (ends && joins[c - 1] == kInside) {  // the first chunk that holds entries of the row
+    u64 lo = 0, hi = c * kPairChunk - 1;  // entry[hi].row == row
+    while (lo < hi) {
+      const u64 mid = (lo + hi) / 2;
+      if (entry[mid].row < row) lo = mid + 1;
+      else hi = mid;
     }
+    from = lo / kPairChunk;
   }
   const bool wide = ends && c - from > 32;
   if (ends && !wide) {
@@ -492,6 +502,7 @@ void build_pair_plan(PairPlan& plan, u64 rows, const i32* pair_rows, u64 pairs, 
   slab.want(plan.terms, pairs);
   slab.want(plan.head, chunks);
   slab.want(plan.tail, chunks);
+  slab.want(plan.joins, chunks);
   slab.want(plan.gap, rows);
   slab.commit(plan.slabs, plan.device);
   const u32 tiles = u32((n + kSortTile - 1) / kSortTile);
@@ -552,10 +563,12 @@ void launch_pair_loss(const PairPlan& p, const PairLoss& a, cudaStream_t s) {
   after_launch("pair loss");
   if (!p.pairs) return;
   const u64 n = 2 * p.pairs, chunks = (n + kPairChunk - 1) / kPairChunk;
-  k_pair_rows<<<u32((chunks + 7) / 8), 256, 0, s>>>(a, p.entry.get(), n, p.terms.get(), p.head.get(), p.tail.get());
+  k_pair_rows<<<u32((chunks + 7) / 8), 256, 0, s>>>(a, p.entry.get(), n, p.terms.get(), p.head.get(), p.tail.get(),
+                                                    p.joins.get());
   after_launch("pair loss");
   if (chunks > 1) {
-    k_pair_joins<<<u32((chunks + 255) / 256), 256, 0, s>>>(a, p.entry.get(), n, p.head.get(), p.tail.get());
+    k_pair_joins<<<u32((chunks + 255) / 256), 256, 0, s>>>(a, p.entry.get(), chunks, p.head.get(), p.tail.get(),
+                                                        p.joins.get());
     after_launch("pair loss");
   }
 }

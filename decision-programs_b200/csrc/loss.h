@@ -98,6 +98,7 @@ struct PairPlan {
   DevBuf<PairEntry> entry;
   DevBuf<float2> terms;        // [pairs] derivative by the preferred score, curvature
   DevBuf<float2> head, tail;   // [chunks] sums of rows that reach over chunks
+  DevBuf<u32> joins;           // [chunks] which of them end there
   DevBuf<float> gap;           // [rows] score - ref
   PairPlan() = default;
   ~PairPlan();  // the plan's device is current

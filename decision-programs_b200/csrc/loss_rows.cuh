@@ -22,16 +22,6 @@
 namespace dp {
 namespace {
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-constexpr float kLog2e = 1.4426950408889634f;
-// e^x.  The difference z - m is taken before the scaling by log2 e: margins of
-// the type's lowest value would overflow if they were scaled first.
-__device__ __forceinline__ float exp_fast(float x) { return ex2(x * kLog2e); }
-
 // Two fp32 numbers in a register pair.
 struct Two {
   u64 v;
@@ -55,7 +45,7 @@ __device__ __forceinline__ Two fma(Two a, Two b, Two c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-__device__ __forceinline__ Two ex2(Two x) {
+__device__ __forceinline__ Two ex2_both(Two x) {
   float a, b;
   x.get(a, b);
   return Two(ex2(a), ex2(b));
@@ -233,7 +223,7 @@ __device__ __forceinline__ void grad_vector(const RowOut<T>& out, u32 j, const u
   Two f[P], e[P];
   Vec<T>::unpack(raw, f);
 #pragma unroll
-  for (int i = 0; i < P; ++i) f[i] = ex2(fma(f[i] + Two(-q.base), Two(kLog2e), Two(q.low)));
+  for (int i = 0; i < P; ++i) f[i] = ex2_both(fma(f[i] + Two(-q.base), Two(kLog2e), Two(q.low)));
 #pragma unroll
   for (int i = 0; i < P; ++i) e[i] = f[i] * Two(-q.c * q.scale);
   out.store(j, Vec<T>::pack(e));
@@ -267,7 +257,7 @@ __device__ __forceinline__ void grad_vectors(const RowOut<T>& out, u32 j, u32 j1
     Vec<T>::unpack(v[u], f);
 #pragma unroll
     for (int i = 0; i < P; ++i)
-      f[i] = ex2(fma(f[i] + Two(-q.base), Two(kLog2e), Two(q.low))) * Two(-q.c * q.scale);
+      f[i] = ex2_both(fma(f[i] + Two(-q.base), Two(kLog2e), Two(q.low))) * Two(-q.c * q.scale);
     v[u] = Vec<T>::pack(f);
   }
   if (out.g16) {
@@ -337,7 +327,7 @@ __device__ __forceinline__ void join_vectors(const uint4 (&v)[U], float& m, floa
     Two f[Vec<T>::P];
     Vec<T>::unpack(v[u], f);
 #pragma unroll
-    for (int i = 0; i < Vec<T>::P; ++i) sum[i & 1] = sum[i & 1] + ex2((f[i] + b) * Two(kLog2e));
+    for (int i = 0; i < Vec<T>::P; ++i) sum[i & 1] = sum[i & 1] + ex2_both((f[i] + b) * Two(kLog2e));
   }
   float x, y;
   (sum[0] + sum[1]).get(x, y);
@@ -362,6 +352,12 @@ __device__ __forceinline__ void cluster_put(float2* at, u32 rank, float2 v) {
   u32 there;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(v.x), "f"(v.y) : "memory");
+}
+__device__ __forceinline__ void cluster_put(i32* at, u32 rank, i32 v) {
+  const u32 here = u32(__cvta_generic_to_shared(at));
+  u32 there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
 }
 constexpr u32 kMaxCluster = 8;
 
@@ -449,7 +445,7 @@ __global__ void __launch_bounds__(256, 4) k_row_loss(RowArgs a) {
   if constexpr (kPolicy) {
     if (!a.out.grad || !in) return;
     const RowOut<T> out(a.out, r, cut.shift);
-    const RowCoef q{c, exp_base(top), 0.f, 1.f / s};
+    const RowCoef q{c, exp_base(top), 0.f, inverse(s)};
     if (c == 0.f) {
       for (u32 j = cut.j0 + lane; j < cut.j1; j += G) out.zero(j);
     } else {
@@ -495,7 +491,8 @@ __device__ __forceinline__ void copy_wait(u32 n) {
   }
 }
 
-// The rows of one cluster in order, their labels read 32 at a time.
+// The rows of one cluster in order, their labels read 32 at a time by each
+// warp for itself: what the copies run ahead by.
 struct RowWalk {
   const i32* label;
   u64 rows, step, r;
@@ -504,10 +501,13 @@ struct RowWalk {
   __device__ __forceinline__ RowWalk(const RowArgs& a, u64 first, u64 clusters)
       : label(a.label), rows(a.m.rows), step(clusters), r(first) {}
   __device__ __forceinline__ bool done() const { return r >= rows; }
+  __device__ __forceinline__ i32 load() const {
+    const u64 mine = r + (threadIdx.x & 31) * step;
+    return mine < rows ? label[mine] : -1;
+  }
   __device__ __forceinline__ i32 here() {
     if (at == 32) {
-      const u64 mine = r + (threadIdx.x & 31) * step;
-      batch = mine < rows ? label[mine] : -1;
+      batch = load();
       at = 0;
     }
     return __shfl_sync(0xffffffffu, batch, at);
@@ -517,6 +517,32 @@ struct RowWalk {
     ++at;
   }
 };
+// The labels that a cluster goes by.  Whether a row takes part decides which
+// barriers its threads meet at, so one warp reads it for all of them: were the
+// labels written while the kernel runs, the results would be of no use, but
+// every thread would still come to the same barriers.
+template <int kWarps>
+__device__ __forceinline__ i32 agreed_label(RowWalk& w, i32 (&labels)[2][32], u32& buffer, u32 rank, u32 blocks) {
+  if constexpr (kWarps == 1) {
+    if (blocks == 1) return w.here();
+  }
+  if (w.at == 32) {
+    buffer ^= 1;  // (slower threads may still read the last 32)
+    w.at = 0;
+    if (rank == 0 && threadIdx.x < 32) {
+      const i32 mine = w.load();
+      for (u32 b = 0; b < blocks; ++b) cluster_put(&labels[buffer][threadIdx.x], b, mine);
+    }
+    if (blocks > 1) {
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+  }
+  return labels[buffer][w.at];
+}
 
 // One block's share [j0, j1) of a row's whole vectors, in groups of NT * U.
 template <class T, int NT, int U>
@@ -539,6 +565,7 @@ __global__ void __launch_bounds__(NT, kPerSM) k_row_loss_ring(RowArgs a, u32 blo
   __shared__ float2 warp_part[2][kWarps];
   __shared__ float2 block_part[2][kMaxCluster];
   __shared__ float row_c[2];
+  __shared__ i32 labels[2][32];
   const u32 t = threadIdx.x, rank = blocks > 1 ? cluster_rank() : 0;
   const u64 first = blocks > 1 ? blockIdx.x / blocks : blockIdx.x;
   const T* const z = static_cast<const T*>(a.m.z);
@@ -593,10 +620,10 @@ __global__ void __launch_bounds__(NT, kPerSM) k_row_loss_ring(RowArgs a, u32 blo
 #pragma unroll 1
   for (int i = 0; i < S; ++i) issue();
 
-  u32 slot = 0, parity = 0;
+  u32 slot = 0, parity = 0, buffer = 0;
   for (RowWalk rows(a, first, clusters); !rows.done(); rows.next()) {
     const u64 r = rows.r;
-    const i32 y = rows.here();
+    const i32 y = agreed_label<kWarps>(rows, labels, buffer, rank, blocks);
     const RowCut<T> cut(z + r * a.m.stride, a.m.classes);
     const RowShare<T, NT, U> share(cut, rank, blocks);
     const u32 groups = share.groups();
@@ -660,7 +687,7 @@ __global__ void __launch_bounds__(NT, kPerSM) k_row_loss_ring(RowArgs a, u32 blo
       }
       parity ^= 1;  // (a row's parts are written while slower threads read the last row's)
       q.base = exp_base(m);
-      q.scale = __frcp_rn(s);
+      q.scale = inverse(s);
     } else {
       skip_row<kPolicy>(a, r, rank == 0 && t == 0);
     }
@@ -707,75 +734,6 @@ __global__ void __launch_bounds__(NT, kPerSM) k_row_loss_ring(RowArgs a, u32 blo
   }
 }
 
-// Few classes: a block stages kTileRows whole rows in shared memory (adjacent
-// threads read adjacent elements, whatever the row length), each thread then
-// takes one row, and the block writes the gradients as it read the margins.
-// Rows lie an odd number of words apart, so that the 32 rows of a warp use
-// the 32 banks.
-constexpr u32 kTileRows = 256, kTileClasses = 32;
-template <class T, bool kPolicy>
-__global__ void __launch_bounds__(kTileRows) k_row_loss_tile(RowArgs a) {
-  extern __shared__ float tile[];
-  __shared__ float4 row_data[kPolicy ? kTileRows : 1];  // c, 1 / s, label
-  const u32 K = a.m.classes, Kp = K | 1u;
-  const u64 r0 = u64(blockIdx.x) * kTileRows;
-  const u32 rows = u32(min(u64(kTileRows), a.m.rows - r0)), n = rows * K;
-  const u32 step_row = kTileRows / K, step_col = kTileRows % K;
-  {
-    const T* z = static_cast<const T*>(a.m.z) + r0 * a.m.stride;
-    u32 row = threadIdx.x / K, col = threadIdx.x % K;
-#pragma unroll 4
-    for (u32 e = threadIdx.x; e < n; e += kTileRows) {
-      tile[row * Kp + col] = to_f32(z[row * a.m.stride + col]);
-      row += step_row;
-      col += step_col;
-      if (col >= K) { col -= K; ++row; }
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x < rows) {
-    const u64 r = r0 + threadIdx.x;
-    float* const z = tile + threadIdx.x * Kp;
-    const i32 y = a.label[r];
-    float c = 0.f, s = 1.f;
-    if (u32(y) < K) {
-      RowScalars x = policy_scalars<kPolicy>(a, r);
-      x.zy = z[y];
-      float m = neg_inf();
-      for (u32 k = 0; k < K; ++k) m = fmaxf(m, z[k]);
-      const float base = exp_base(m);
-      s = 0.f;
-      for (u32 k = 0; k < K; ++k) {
-        const float e = exp_fast(z[k] - base);
-        s += e;
-        if constexpr (kPolicy) z[k] = e;
-      }
-      c = finish_row<kPolicy>(a, r, x, m, s, true);
-    } else {
-      skip_row<kPolicy>(a, r, true);
-    }
-    if constexpr (kPolicy) row_data[threadIdx.x] = make_float4(c, 1.f / s, __int_as_float(y), 0.f);
-  }
-  if constexpr (kPolicy) {
-    if (!a.out.grad) return;
-    __syncthreads();
-    T* const g = static_cast<T*>(a.out.grad) + r0 * a.out.grad_stride;
-    float* const h = a.out.hess ? a.out.hess + r0 * a.out.hess_stride : nullptr;
-    u32 row = threadIdx.x / K, col = threadIdx.x % K;
-#pragma unroll 4
-    for (u32 e = threadIdx.x; e < n; e += kTileRows) {
-      const float4 d = row_data[row];
-      const float p = tile[row * Kp + col] * d.y;
-      const bool none = d.x == 0.f;
-      g[row * a.out.grad_stride + col] = from_f32<T>(none ? 0.f : margin_grad(d.x, p, col == u32(__float_as_int(d.z))));
-      if (h) h[row * a.out.hess_stride + col] = none ? 0.f : margin_hess(d.x, p);
-      row += step_row;
-      col += step_col;
-      if (col >= K) { col -= K; ++row; }
-    }
-  }
-}
-
 // ---- the backward pass alone: the row's norm is given, so every element is
 // on its own.
 
@@ -818,40 +776,136 @@ __global__ void __launch_bounds__(256) k_log_prob_grad(GradArgs a, u32 pieces) {
   if (labels) grad_label(out, cut, y, zy, q);
 }
 
-// Few classes: a block takes kTileRows rows, adjacent threads adjacent elements.
-template <class T>
-__global__ void __launch_bounds__(kTileRows) k_log_prob_grad_tile(GradArgs a) {
-  __shared__ float4 row_data[kTileRows];  // c, norm, label
-  const u32 K = a.m.classes;
-  const u64 r0 = u64(blockIdx.x) * kTileRows;
-  const u32 rows = u32(min(u64(kTileRows), a.m.rows - r0)), n = rows * K;
-  if (threadIdx.x < rows) {
-    const u64 r = r0 + threadIdx.x;
-    const i32 y = a.label[r];
-    const float2 nm = a.norm[r];
-    row_data[threadIdx.x] = make_float4(grad_weight(a, r, y, nm), nm.x, nm.y, __int_as_float(y));
-  }
-  __syncthreads();
-  const T* const z = static_cast<const T*>(a.m.z) + r0 * a.m.stride;
-  T* const g = static_cast<T*>(a.out.grad) + r0 * a.out.grad_stride;
-  float* const h = a.out.hess ? a.out.hess + r0 * a.out.hess_stride : nullptr;
-  const u32 step_row = kTileRows / K, step_col = kTileRows % K;
-  u32 row = threadIdx.x / K, col = threadIdx.x % K;
+// ---- few classes: a block stages whole rows in shared memory, as they lie in
+// memory, each thread takes one row into registers, puts its gradient back in
+// the row's place, and the block copies the gradients out.  So memory is read
+// and written in whole lines whatever the row length, and a row costs one
+// thread's instructions.  The threads of a warp would meet in the same banks
+// where the row length shares a factor with the 32 banks: each begins its row
+// at a place of its own (`turn`) and goes round.
+struct TileArgs {
+  RowArgs row;
+  const float2* norm;    // the backward pass alone: the rows' norms
+  const float* weight;   // and the loss's derivatives
+};
+enum TileMode { kTileLogProb, kTilePolicy, kTileGrad };
+constexpr u32 kTileClasses = 64;
+
+// Copies `rows` rows of K elements between memory (`stride` apart) and a tile
+// without gaps; whole vectors when the rows have no gaps either.
+template <class U, bool kIn>
+__device__ __forceinline__ void copy_rows(U* tile, U* mem, u32 rows, u32 K, u64 stride) {
+  const u32 n = rows * K;
+  if (stride == K && (reinterpret_cast<std::uintptr_t>(mem) & 15) == 0) {
+    constexpr u32 N = 16 / sizeof(U);
+    uint4 *const a = reinterpret_cast<uint4*>(tile), *const b = reinterpret_cast<uint4*>(mem);
 #pragma unroll 4
-  for (u32 e = threadIdx.x; e < n; e += kTileRows) {
-    const float4 d = row_data[row];
-    float gv = 0.f, hv = 0.f;
-    if (d.x != 0.f) {
-      const float p = exp_fast((to_f32(z[row * a.m.stride + col]) - d.y) - d.z);
-      gv = margin_grad(d.x, p, col == u32(__float_as_int(d.w)));
-      hv = margin_hess(d.x, p);
+    for (u32 j = threadIdx.x; j < n / N; j += blockDim.x) {
+      if (kIn) a[j] = b[j];
+      else b[j] = a[j];
     }
-    g[row * a.out.grad_stride + col] = from_f32<T>(gv);
-    if (h) h[row * a.out.hess_stride + col] = hv;
-    row += step_row;
-    col += step_col;
-    if (col >= K) { col -= K; ++row; }
+    const u32 e = n / N * N + threadIdx.x;  // (fewer elements than threads are left)
+    if (e < n) {
+      if (kIn) tile[e] = mem[e];
+      else mem[e] = tile[e];
+    }
+  } else {
+    const u32 step_row = blockDim.x / K, step_col = blockDim.x % K;
+    u32 row = threadIdx.x / K, col = threadIdx.x % K;
+#pragma unroll 4
+    for (u32 e = threadIdx.x; e < n; e += blockDim.x) {
+      if (kIn) tile[e] = mem[row * stride + col];
+      else mem[row * stride + col] = tile[e];
+      row += step_row;
+      col += step_col;
+      if (col >= K) { col -= K; ++row; }
+    }
   }
+}
+
+// NT rows a block; KT: the most classes, which fit a thread's registers.
+template <class T, TileMode kMode, int KT, int NT>
+__global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread) {
+  extern __shared__ uint4 tile16[];
+  const RowArgs& a = t.row;
+  const u32 K = a.m.classes;
+  T* const tile = reinterpret_cast<T*>(tile16);
+  float* const htile = reinterpret_cast<float*>(tile16 + (u64(NT) * K * sizeof(T) + 15) / 16);
+  const u64 r0 = u64(blockIdx.x) * NT, r = r0 + threadIdx.x;
+  const u32 rows = u32(min(u64(NT), a.m.rows - r0));
+  const bool in = threadIdx.x < rows;
+  const i32 y = in ? a.label[r] : -1;
+  const bool live = u32(y) < K;
+  RowScalars x;
+  float2 norm = make_float2(0.f, 0.f);
+  float c = 0.f;
+  if (live) {
+    x = policy_scalars<kMode == kTilePolicy>(a, r);
+    if constexpr (kMode == kTileGrad) {
+      norm = t.norm[r];
+      if (!(norm.x == neg_inf() && norm.y == 0.f)) c = t.weight[r];
+    }
+  }
+  copy_rows<T, true>(tile, const_cast<T*>(static_cast<const T*>(a.m.z)) + r0 * a.m.stride, rows, K, a.m.stride);
+  __syncthreads();
+  const bool backward = kMode == kTileGrad || (kMode == kTilePolicy && a.out.grad != nullptr);
+  if (in) {
+    T* const mine = tile + threadIdx.x * K;
+    const u32 turn = (threadIdx.x & 31) / spread * (4 / u32(sizeof(T))) % K;
+    float z[KT];
+    float base = norm.x, low = -norm.y * kLog2e, scale = 1.f;
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        if (u32(k) < K) {
+          const u32 at = turn + k;
+          z[k] = to_f32(mine[at < K ? at : at - K]);
+        } else {
+          z[k] = neg_inf();
+        }
+      }
+      if constexpr (kMode != kTileGrad) {
+        x.zy = to_f32(mine[y]);
+        float m = z[0], s = 0.f;
+#pragma unroll
+        for (int k = 1; k < KT; ++k)
+          if (u32(k) < K) m = fmaxf(m, z[k]);
+        base = exp_base(m);
+        low = 0.f;
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+          if (u32(k) < K) {
+            z[k] = exp_fast(z[k] - base);
+            s += z[k];
+          }
+        }
+        c = finish_row<kMode == kTilePolicy>(a, r, x, m, s, true);
+        scale = inverse(s);
+      }
+    } else if constexpr (kMode != kTileGrad) {
+      skip_row<kMode == kTilePolicy>(a, r, true);
+    }
+    if (backward) {
+      const bool none = c == 0.f;
+      float* const mine_h = htile + threadIdx.x * K;
+      const bool hess = a.out.hess != nullptr;
+      const float up = fabsf(c);
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        if (u32(k) < K) {
+          u32 at = turn + k;
+          at = at < K ? at : at - K;
+          const float p = kMode == kTileGrad ? ex2(fmaf(z[k] - base, kLog2e, low)) : z[k] * scale;
+          mine[at] = from_f32<T>(none ? 0.f : margin_grad(c, p, at == u32(y)));
+          if (hess) mine_h[at] = none ? 0.f : up * fmaxf(2.f * p * (1.f - p), 1e-16f);
+        }
+      }
+    }
+  }
+  if (!backward) return;
+  __syncthreads();
+  copy_rows<T, false>(tile, static_cast<T*>(a.out.grad) + r0 * a.out.grad_stride, rows, K, a.out.grad_stride);
+  if (a.out.hess) copy_rows<float, false>(htile, a.out.hess + r0 * a.out.hess_stride, rows, K, a.out.hess_stride);
 }
 
 // ---- launches ---------------------------------------------------------------
@@ -865,6 +919,27 @@ inline u32 grid_of(u64 blocks) {
 template <class T>
 u32 row_vectors(const Margins& m) {
   return m.classes / u32(16 / sizeof(T));
+}
+
+template <class T, TileMode kMode, int KT, int NT>
+void launch_tile_of(const TileArgs& t, cudaStream_t s) {
+  const u64 K = t.row.m.classes, size = (NT * K * sizeof(T) + 15) / 16 * 16 + (t.row.out.hess ? NT * K * 4 : 0);
+  auto* const kernel = k_row_tile<T, kMode, KT, NT>;
+  if (size > 48 * 1024) DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(size)));
+  // lanes `spread` apart would meet in a bank: the row length's common factor with the banks
+  const u32 words = u32(K * sizeof(T) % 4 ? 1 : K * sizeof(T) / 4);
+  u32 spread = 32;
+  while (spread > 1 && words % (64 / spread) == 0) spread /= 2;
+  kernel<<<grid_of((t.row.m.rows + NT - 1) / NT), NT, size, s>>>(t, spread);
+}
+template <class T, TileMode kMode>
+void launch_tile(const TileArgs& t, cudaStream_t s) {
+  const u32 K = t.row.m.classes;
+  if (K <= 4) launch_tile_of<T, kMode, 4, 256>(t, s);
+  else if (K <= 8) launch_tile_of<T, kMode, 8, 256>(t, s);
+  else if (K <= 16) launch_tile_of<T, kMode, 16, 256>(t, s);
+  else if (K <= 32) launch_tile_of<T, kMode, 32, 128>(t, s);
+  else launch_tile_of<T, kMode, 64, 128>(t, s);
 }
 
 template <class T, bool kPolicy, int G>
@@ -929,8 +1004,7 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
   constexpr u32 V = 8;  // most vectors a lane holds
   const u32 K = a.m.classes, nvec = row_vectors<T>(a.m);
   if (K <= kTileClasses) {
-    const size_t shared = size_t(kTileRows) * (K | 1u) * sizeof(float);
-    k_row_loss_tile<T, kPolicy><<<grid_of((a.m.rows + kTileRows - 1) / kTileRows), kTileRows, shared, s>>>(a);
+    launch_tile<T, kPolicy ? kTilePolicy : kTileLogProb>(TileArgs{a, nullptr, nullptr}, s);
   } else if (nvec <= 8 * V) {
     launch_lanes<T, kPolicy, 8>(a, (nvec + 7) / 8, s);
   } else if (nvec <= 32 * V) {
@@ -971,7 +1045,11 @@ void launch_grad_of(const GradArgs& a, cudaStream_t s) {
   const u32 nvec = row_vectors<T>(a.m);
   constexpr u32 U = 4;
   if (a.m.classes <= kTileClasses) {
-    k_log_prob_grad_tile<T><<<grid_of((rows + kTileRows - 1) / kTileRows), kTileRows, 0, s>>>(a);
+    RowArgs row{};
+    row.m = a.m;
+    row.label = a.label;
+    row.out = a.out;
+    launch_tile<T, kTileGrad>(TileArgs{row, a.norm, a.weight}, s);
   } else if (nvec <= 8 * U) {
     k_log_prob_grad<T, 8, U><<<grid_of((rows + 31) / 32), 256, 0, s>>>(a, 1u);
   } else if (nvec <= 32 * U * 2) {

@@ -485,50 +485,48 @@ def _vector(t, n: int, dtype, device, name: str, optional: bool = False, shape=N
     if t is None and optional:
         return None
     shape = (n,) if shape is None else shape
-    _need(tuple(t.shape) == shape, f"{name} must have shape {list(shape)}, got {list(t.shape)}")
-    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    _need(t.device == device, f"{name} must be on {device}, got {t.device}")
-    return t.contiguous()
+    if t.shape != shape:
+        raise DPError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise DPError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise DPError(f"{name} must be on {device}, got {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """The device of a call's tensors made current, and its torch stream."""
+def _elsewhere(device) -> bool:
+    """Whether a call has to make `device`, its tensors' one, current first."""
+    import torch
+    _need(device.type == "cuda", "the tensors must be CUDA tensors")
+    return device.index != torch.cuda.current_device()
 
-    def __init__(self, device):
-        import torch
-        _need(device.type == "cuda", "the tensors must be CUDA tensors")
-        self._guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-        self.stream = torch.cuda.current_stream(device).cuda_stream
 
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _stream() -> int:
+    import torch
+    return torch.cuda.current_stream().cuda_stream
 
 
 def _rows_of(t, name: str):
     """(pointer, row stride) of a [R, K] tensor whose classes are adjacent."""
-    rows, classes = t.shape
-    _need(classes <= 1 or t.stride(1) == 1, f"{name}: the classes of a row must be adjacent in memory")
-    return t.data_ptr(), (t.stride(0) if rows > 1 else max(classes, t.stride(0)))
+    (rows, classes), (apart, step) = t.shape, t.stride()
+    if classes > 1 and step != 1:
+        raise DPError(f"{name}: the classes of a row must be adjacent in memory")
+    return t.data_ptr(), (apart if rows > 1 else max(classes, apart))
 
 
 def _margins(margin):
     """The leading arguments of a call on class margins [R, K]."""
     import torch
-    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
     _need(margin.dim() == 2, "margin must be [rows, classes]")
-    _need(margin.dtype in types, "margin must be float32, float16 or bfloat16")
+    dtype = margin.dtype
+    kind = 2 if dtype == torch.bfloat16 else 0 if dtype == torch.float32 else 1
+    _need(kind != 1 or dtype == torch.float16, "margin must be float32, float16 or bfloat16")
     ptr, stride = _rows_of(margin, "margin")
-    return types[margin.dtype], ptr, margin.shape[0], margin.shape[1], stride
+    return kind, ptr, margin.shape[0], margin.shape[1], stride
 
 
 def _grad_out(margin, grad, hess):
@@ -539,8 +537,10 @@ def _grad_out(margin, grad, hess):
     else:
         _need(grad.shape == margin.shape and grad.dtype == margin.dtype and grad.device == margin.device,
               "grad must have the margins' shape, type and device")
-    hess = torch.empty(margin.shape, dtype=torch.float32, device=margin.device) if hess else None
-    return grad, hess, (*_rows_of(grad, "grad"), *(_rows_of(hess, "hess") if hess is not None else (None, 0)))
+    if not hess:
+        return grad, None, (*_rows_of(grad, "grad"), None, 0)
+    hess = torch.empty(margin.shape, dtype=torch.float32, device=margin.device)
+    return grad, hess, (*_rows_of(grad, "grad"), *_rows_of(hess, "hess"))
 
 
 def log_prob(margin, label):
@@ -549,13 +549,16 @@ def log_prob(margin, label):
     [R, K] float32, float16 or bfloat16 (row stride allowed); label: int32
     [R], rows whose label is not a class are skipped."""
     import torch
+    dev = margin.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return log_prob(margin, label)
     m = _margins(margin)
-    rows, dev = margin.shape[0], margin.device
-    with _on(dev) as stream:
-        label = _vector(label, rows, torch.int32, dev, "label")
-        out = torch.empty(rows, dtype=torch.float32, device=dev)
-        norm = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-        check(lib().dp_log_prob(*m, label.data_ptr(), out.data_ptr(), norm.data_ptr(), stream))
+    rows = m[2]
+    label = _vector(label, rows, torch.int32, dev, "label")
+    out = torch.empty(rows, dtype=torch.float32, device=dev)
+    norm = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+    check(lib().dp_log_prob(*m, label.data_ptr(), out.data_ptr(), norm.data_ptr(), _stream()))
     return out, norm
 
 
@@ -564,14 +567,17 @@ def log_prob_grad(margin, label, norm, weight, grad=None, hess: bool = False):
     derivative of a loss by each log-probability.  grad: a tensor to write to
     (the margins themselves included); hess: the diagonal curvature too."""
     import torch
+    dev = margin.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return log_prob_grad(margin, label, norm, weight, grad, hess)
     m = _margins(margin)
-    rows, dev = margin.shape[0], margin.device
-    with _on(dev) as stream:
-        label = _vector(label, rows, torch.int32, dev, "label")
-        norm = _vector(norm, rows, torch.float32, dev, "norm", shape=(rows, 2))
-        weight = _vector(weight, rows, torch.float32, dev, "weight")
-        grad, hess, out = _grad_out(margin, grad, hess)
-        check(lib().dp_log_prob_grad(*m, label.data_ptr(), norm.data_ptr(), weight.data_ptr(), *out, stream))
+    rows = m[2]
+    label = _vector(label, rows, torch.int32, dev, "label")
+    norm = _vector(norm, rows, torch.float32, dev, "norm", shape=(rows, 2))
+    weight = _vector(weight, rows, torch.float32, dev, "weight")
+    grad, hess, out = _grad_out(margin, grad, hess)
+    check(lib().dp_log_prob_grad(*m, label.data_ptr(), norm.data_ptr(), weight.data_ptr(), *out, _stream()))
     return grad, hess
 
 
@@ -583,33 +589,38 @@ def policy_loss(margin, label, old_log_prob, advantage, ref_log_prob=None, weigh
     True, a tensor to write to (the margins themselves included), or False for
     the forward pass alone; hess: the diagonal curvature too."""
     import torch
+    dev = margin.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return policy_loss(margin, label, old_log_prob, advantage, ref_log_prob, weight, clip, kl, grad, hess)
     m = _margins(margin)
-    rows, dev = margin.shape[0], margin.device
-    with _on(dev) as stream:
-        label = _vector(label, rows, torch.int32, dev, "label")
-        old_log_prob = _vector(old_log_prob, rows, torch.float32, dev, "old_log_prob")
-        advantage = _vector(advantage, rows, torch.float32, dev, "advantage")
-        ref_log_prob = _vector(ref_log_prob, rows, torch.float32, dev, "ref_log_prob", optional=True)
-        weight = _vector(weight, rows, torch.float32, dev, "weight", optional=True)
-        _need(grad is not False or not hess, "hess is written with a gradient: grad is False")
-        loss = torch.empty(rows, dtype=torch.float32, device=dev)
-        logp = torch.empty(rows, dtype=torch.float32, device=dev)
-        grad, hess, out = (None, None, (None, 0, None, 0)) if grad is False else _grad_out(margin, grad, hess)
-        check(lib().dp_policy_loss(*m, label.data_ptr(), old_log_prob.data_ptr(), _ptr(ref_log_prob),
-                                   advantage.data_ptr(), _ptr(weight), clip[0], clip[1], kl, loss.data_ptr(),
-                                   logp.data_ptr(), *out, stream))
+    rows, f32 = m[2], torch.float32
+    label = _vector(label, rows, torch.int32, dev, "label")
+    old_log_prob = _vector(old_log_prob, rows, f32, dev, "old_log_prob")
+    advantage = _vector(advantage, rows, f32, dev, "advantage")
+    ref_log_prob = _vector(ref_log_prob, rows, f32, dev, "ref_log_prob", optional=True)
+    weight = _vector(weight, rows, f32, dev, "weight", optional=True)
+    _need(grad is not False or not hess, "hess is written with a gradient: grad is False")
+    loss = torch.empty(rows, dtype=f32, device=dev)
+    logp = torch.empty(rows, dtype=f32, device=dev)
+    grad, hess, out = (None, None, (None, 0, None, 0)) if grad is False else _grad_out(margin, grad, hess)
+    check(lib().dp_policy_loss(*m, label.data_ptr(), old_log_prob.data_ptr(), _ptr(ref_log_prob),
+                               advantage.data_ptr(), _ptr(weight), clip[0], clip[1], kl, loss.data_ptr(),
+                               logp.data_ptr(), *out, _stream()))
     return PolicyLoss(loss, logp, grad, hess)
 
 
 def _pair_tensors(score, ref_score, weight, pairs: int, hess: bool):
     import torch
+    f32, dev = torch.float32, score.device
     _need(score.dim() == 1, "score must be a vector")
-    rows, dev = score.shape[0], score.device
-    score = _vector(score, rows, torch.float32, dev, "score")
-    ref_score = _vector(ref_score, rows, torch.float32, dev, "ref_score", optional=True)
-    weight = _vector(weight, pairs, torch.float32, dev, "weight", optional=True)
-    new = lambda n: torch.empty(n, dtype=torch.float32, device=dev)  # noqa: E731
-    return score, ref_score, weight, PreferenceLoss(new(pairs), new(rows), new(rows) if hess else None)
+    rows = score.shape[0]
+    score = _vector(score, rows, f32, dev, "score")
+    ref_score = _vector(ref_score, rows, f32, dev, "ref_score", optional=True)
+    weight = _vector(weight, pairs, f32, dev, "weight", optional=True)
+    out = PreferenceLoss(torch.empty(pairs, dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev),
+                         torch.empty(rows, dtype=f32, device=dev) if hess else None)
+    return score, ref_score, weight, out
 
 
 def preference_loss(score, ref_score=None, item_begin=None, weight=None, beta: float = 1.0, smoothing: float = 0.0,
@@ -620,18 +631,20 @@ def preference_loss(score, ref_score=None, item_begin=None, weight=None, beta: f
     [P] fp32."""
     import torch
     dev = score.device
-    with _on(dev) as stream:
-        if item_begin is None:
-            _need(score.dim() == 1 and score.shape[0] % 2 == 0, "without item offsets score holds pairs of rows")
-            pairs = score.shape[0] // 2
-        else:
-            _need(item_begin.dim() == 1 and item_begin.shape[0] % 2 == 1, "item_begin must hold 2 * pairs + 1 offsets")
-            pairs = item_begin.shape[0] // 2
-            item_begin = _vector(item_begin, 2 * pairs + 1, torch.int64, dev, "item_begin")
-        score, ref_score, weight, out = _pair_tensors(score, ref_score, weight, pairs, hess)
-        check(lib().dp_preference_loss(score.shape[0], _ptr(item_begin), pairs, score.data_ptr(), _ptr(ref_score),
-                                       _ptr(weight), beta, smoothing, out.loss.data_ptr(), out.grad.data_ptr(),
-                                       _ptr(out.hess), stream))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return preference_loss(score, ref_score, item_begin, weight, beta, smoothing, hess)
+    if item_begin is None:
+        _need(score.dim() == 1 and score.shape[0] % 2 == 0, "without item offsets score holds pairs of rows")
+        pairs = score.shape[0] // 2
+    else:
+        _need(item_begin.dim() == 1 and item_begin.shape[0] % 2 == 1, "item_begin must hold 2 * pairs + 1 offsets")
+        pairs = item_begin.shape[0] // 2
+        item_begin = _vector(item_begin, 2 * pairs + 1, torch.int64, dev, "item_begin")
+    score, ref_score, weight, out = _pair_tensors(score, ref_score, weight, pairs, hess)
+    check(lib().dp_preference_loss(score.shape[0], _ptr(item_begin), pairs, score.data_ptr(), _ptr(ref_score),
+                                   _ptr(weight), beta, smoothing, out.loss.data_ptr(), out.grad.data_ptr(),
+                                   _ptr(out.hess), _stream()))
     return out
 
 
@@ -644,21 +657,29 @@ class PreferencePairs:
         import torch
         self.handle = C.c_void_p()
         self.pairs, self.rows, self.device = pairs.shape[0], int(rows), pairs.device
-        with _on(pairs.device) as stream:
-            pairs = _vector(pairs, self.pairs, torch.int32, pairs.device, "pairs", shape=(self.pairs, 2))
-            check(lib().dp_preference_prepare(self.rows, pairs.data_ptr(), self.pairs, stream, C.byref(self.handle)))
+        _need(self.device.type == "cuda", "the tensors must be CUDA tensors")
+        with torch.cuda.device(self.device):
+            pairs = _vector(pairs, self.pairs, torch.int32, self.device, "pairs", shape=(self.pairs, 2))
+            check(lib().dp_preference_prepare(self.rows, pairs.data_ptr(), self.pairs, _stream(),
+                                              C.byref(self.handle)))
 
     def loss(self, score, ref_score=None, weight=None, beta: float = 1.0, smoothing: float = 0.0,
              hess: bool = False) -> PreferenceLoss:
-        """The preference loss of score [rows] fp32, with weight [P]."""
+        """The preference loss of score [rows] fp32, with weight [P].  The runs
+        of one plan share its workspace: order them if they are on different
+        streams."""
+        import torch
         _need(bool(self.handle), "the pairs have been freed")
-        _need(tuple(score.shape) == (self.rows,), f"score must have shape {[self.rows]}, got {list(score.shape)}")
-        _need(score.device == self.device, f"score must be on {self.device}, got {score.device}")
-        with _on(self.device) as stream:
-            score, ref_score, weight, out = _pair_tensors(score, ref_score, weight, self.pairs, hess)
-            check(lib().dp_preference_run(self.handle, score.data_ptr(), _ptr(ref_score), _ptr(weight), beta,
-                                          smoothing, out.loss.data_ptr(), out.grad.data_ptr(), _ptr(out.hess),
-                                          stream))
+        if score.shape != (self.rows,):
+            raise DPError(f"score must have shape {[self.rows]}, got {list(score.shape)}")
+        if score.device != self.device:
+            raise DPError(f"score must be on {self.device}, got {score.device}")
+        if _elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return self.loss(score, ref_score, weight, beta, smoothing, hess)
+        score, ref_score, weight, out = _pair_tensors(score, ref_score, weight, self.pairs, hess)
+        check(lib().dp_preference_run(self.handle, score.data_ptr(), _ptr(ref_score), _ptr(weight), beta, smoothing,
+                                      out.loss.data_ptr(), out.grad.data_ptr(), _ptr(out.hess), _stream()))
         return out
 
     def free(self) -> None:
