@@ -776,13 +776,13 @@ __global__ void __launch_bounds__(256) k_log_prob_grad(GradArgs a, u32 pieces) {
   if (labels) grad_label(out, cut, y, zy, q);
 }
 
-// ---- few classes: a block stages whole rows in shared memory, as they lie in
-// memory, each thread takes one row into registers, puts its gradient back in
-// the row's place, and the block copies the gradients out.  So memory is read
-// and written in whole lines whatever the row length, and a row costs one
-// thread's instructions.  The threads of a warp would meet in the same banks
-// where the row length shares a factor with the 32 banks: each begins its row
-// at a place of its own (`turn`) and goes round.
+// ---- few classes: one thread a row, the row in its registers.  Rows that are
+// a power of two of bytes, up to 64, and lie on its boundaries are moved by
+// the thread itself; others go through shared memory, where a block stages
+// them as they lie in memory, each thread puts its gradient back in its row's
+// place, and the block copies the gradients out: memory is read and written in
+// whole lines whatever the row length.  A row costs one thread about a hundred
+// instructions and ten to twenty a class.
 struct TileArgs {
   RowArgs row;
   const float2* norm;    // the backward pass alone: the rows' norms
@@ -823,14 +823,70 @@ __device__ __forceinline__ void copy_rows(U* tile, U* mem, u32 rows, u32 K, u64 
   }
 }
 
-// NT rows a block; KT: the most classes, which fit a thread's registers.
-template <class T, TileMode kMode, int KT, int NT>
+// Turns a row's margins (-inf past its K classes) into probabilities and
+// writes the row's results; c: in, the loss's derivative where it is given;
+// out, the one to go by, 0 for a row without gradient.
+template <TileMode kMode, int KT>
+__device__ __forceinline__ void tile_row(const TileArgs& t, u64 r, u32 K, bool live, RowScalars& x, float2 norm, float& c,
+                                         float (&z)[KT]) {
+  constexpr int kStep = KT < 4 ? KT : 4;
+  if (!live) {
+    if constexpr (kMode != kTileGrad) skip_row<kMode == kTilePolicy>(t.row, r, true);
+    c = 0.f;
+    return;
+  }
+  float m = norm.x, low = -norm.y * kLog2e;
+  if constexpr (kMode != kTileGrad) {
+    m = z[0];
+#pragma unroll
+    for (int k = 1; k < KT; ++k) m = fmaxf(m, z[k]);
+    low = 0.f;
+  }
+  const Two base(-exp_base(m));
+  Two sum(0.f);
+#pragma unroll
+  for (int k4 = 0; k4 < KT; k4 += kStep) {
+    if (KT <= 8 || u32(k4) < K) {
+#pragma unroll
+      for (int k = k4; k < k4 + kStep; k += 2) {
+        if constexpr (KT == 1) {
+          z[0] = ex2(fmaf(z[0] - exp_base(m), kLog2e, low));
+          sum = sum + Two(z[0], 0.f);
+        } else {
+          const Two e = ex2_both(fma(Two(z[k], z[k + 1]) + base, Two(kLog2e), Two(low)));
+          sum = sum + e;
+          e.get(z[k], z[k + 1]);
+        }
+      }
+    }
+  }
+  if constexpr (kMode != kTileGrad) {
+    float s, odd;
+    sum.get(s, odd);
+    s += odd;
+    c = finish_row<kMode == kTilePolicy>(t.row, r, x, m, s, true);
+    const float scale = inverse(s);
+#pragma unroll
+    for (int k = 0; k < KT; ++k) z[k] *= scale;
+  }
+}
+// The row's curvature by one probability.
+__device__ __forceinline__ float tile_hess(float up, float least, float p) {
+  const float h = (1.f - p) * p * (up + up);
+  return h < least ? least : h;  // (a NaN stays one)
+}
+
+// NT rows a block; KT: the most classes.  kTurn: row lengths that share a
+// factor of 8 or more with the 32 banks, where the threads of a warp would
+// read and write in few of them: each begins its row at a place of its own
+// and goes round.
+template <class T, TileMode kMode, int KT, int NT, bool kTurn>
 __global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread) {
   extern __shared__ uint4 tile16[];
   const RowArgs& a = t.row;
   const u32 K = a.m.classes;
   T* const tile = reinterpret_cast<T*>(tile16);
-  float* const htile = reinterpret_cast<float*>(tile16 + (u64(NT) * K * sizeof(T) + 15) / 16);
+  float* const htile = reinterpret_cast<float*>(tile16 + (NT * K * u32(sizeof(T)) + 15) / 16);
   const u64 r0 = u64(blockIdx.x) * NT, r = r0 + threadIdx.x;
   const u32 rows = u32(min(u64(NT), a.m.rows - r0));
   const bool in = threadIdx.x < rows;
@@ -851,61 +907,93 @@ __global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread) {
   const bool backward = kMode == kTileGrad || (kMode == kTilePolicy && a.out.grad != nullptr);
   if (in) {
     T* const mine = tile + threadIdx.x * K;
-    const u32 turn = (threadIdx.x & 31) / spread * (4 / u32(sizeof(T))) % K;
+    const u32 turn = kTurn ? (threadIdx.x & 31) / spread * (4 / u32(sizeof(T))) : 0;
+    auto place = [&](u32 k) {  // the class that register k holds
+      const u32 at = turn + k;
+      return kTurn && at >= K ? at - K : at;
+    };
     float z[KT];
-    float base = norm.x, low = -norm.y * kLog2e, scale = 1.f;
-    if (live) {
 #pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        if (u32(k) < K) {
-          const u32 at = turn + k;
-          z[k] = to_f32(mine[at < K ? at : at - K]);
-        } else {
-          z[k] = neg_inf();
-        }
-      }
-      if constexpr (kMode != kTileGrad) {
-        x.zy = to_f32(mine[y]);
-        float m = z[0], s = 0.f;
-#pragma unroll
-        for (int k = 1; k < KT; ++k)
-          if (u32(k) < K) m = fmaxf(m, z[k]);
-        base = exp_base(m);
-        low = 0.f;
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          if (u32(k) < K) {
-            z[k] = exp_fast(z[k] - base);
-            s += z[k];
-          }
-        }
-        c = finish_row<kMode == kTilePolicy>(a, r, x, m, s, true);
-        scale = inverse(s);
-      }
-    } else if constexpr (kMode != kTileGrad) {
-      skip_row<kMode == kTilePolicy>(a, r, true);
-    }
+    for (int k = 0; k < KT; ++k) z[k] = u32(k) < K ? to_f32(mine[place(k)]) : neg_inf();
+    if (kMode != kTileGrad && live) x.zy = to_f32(mine[y]);
+    tile_row<kMode, KT>(t, r, K, live, x, norm, c, z);
     if (backward) {
-      const bool none = c == 0.f;
       float* const mine_h = htile + threadIdx.x * K;
-      const bool hess = a.out.hess != nullptr;
-      const float up = fabsf(c);
+      const bool none = c == 0.f, hess = a.out.hess != nullptr;
+      const float up = fabsf(c), least = up * 1e-16f, down = -c;
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         if (u32(k) < K) {
-          u32 at = turn + k;
-          at = at < K ? at : at - K;
-          const float p = kMode == kTileGrad ? ex2(fmaf(z[k] - base, kLog2e, low)) : z[k] * scale;
-          mine[at] = from_f32<T>(none ? 0.f : margin_grad(c, p, at == u32(y)));
-          if (hess) mine_h[at] = none ? 0.f : up * fmaxf(2.f * p * (1.f - p), 1e-16f);
+          const u32 at = place(k);
+          mine[at] = from_f32<T>(none ? 0.f : down * z[k]);
+          if (hess) mine_h[at] = none ? 0.f : tile_hess(up, least, z[k]);
+          if (at == u32(y)) c = none ? 0.f : c - c * z[k];
         }
       }
+      if (!none) mine[y] = from_f32<T>(c);
     }
   }
   if (!backward) return;
   __syncthreads();
   copy_rows<T, false>(tile, static_cast<T*>(a.out.grad) + r0 * a.out.grad_stride, rows, K, a.out.grad_stride);
   if (a.out.hess) copy_rows<float, false>(htile, a.out.hess + r0 * a.out.hess_stride, rows, K, a.out.hess_stride);
+}
+
+// A row of B bytes between registers and memory on its boundaries.
+template <int B>
+struct RowBytes {
+  static constexpr int kWord = B < 16 ? B : 16;
+  using Word = typename std::conditional<B == 4, u32, typename std::conditional<B == 8, uint2, uint4>::type>::type;
+  Word w[B / kWord];
+  __device__ __forceinline__ void load(const void* p) {
+#pragma unroll
+    for (int i = 0; i < B / kWord; ++i) w[i] = static_cast<const Word*>(p)[i];
+  }
+  __device__ __forceinline__ void store(void* p) const {
+#pragma unroll
+    for (int i = 0; i < B / kWord; ++i) static_cast<Word*>(p)[i] = w[i];
+  }
+};
+template <class T, TileMode kMode, int K>
+__global__ void __launch_bounds__(256) k_row_thread(TileArgs t) {
+  const RowArgs& a = t.row;
+  const u64 r = u64(blockIdx.x) * 256 + threadIdx.x;
+  if (r >= a.m.rows) return;
+  const i32 y = a.label[r];
+  const bool live = u32(y) < u32(K);
+  RowBytes<K * int(sizeof(T))> raw;
+  T v[K];
+  float z[K];
+  RowScalars x;
+  float2 norm = make_float2(0.f, 0.f);
+  float c = 0.f;
+  raw.load(static_cast<const T*>(a.m.z) + r * a.m.stride);
+  x = policy_scalars<kMode == kTilePolicy>(a, r);
+  if constexpr (kMode == kTileGrad) {
+    norm = t.norm[r];
+    if (!(norm.x == neg_inf() && norm.y == 0.f)) c = t.weight[r];
+  }
+  memcpy(v, &raw, sizeof v);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    z[k] = to_f32(v[k]);
+    if (k == y) x.zy = z[k];
+  }
+  tile_row<kMode, K>(t, r, K, live, x, norm, c, z);
+  if (kMode == kTileLogProb || (kMode == kTilePolicy && !a.out.grad)) return;
+  const bool none = c == 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = from_f32<T>(none ? 0.f : margin_grad(c, z[k], k == y));
+  memcpy(&raw, v, sizeof v);
+  raw.store(static_cast<T*>(a.out.grad) + r * a.out.grad_stride);
+  if (a.out.hess) {
+    const float up = fabsf(c), least = up * 1e-16f;
+    RowBytes<K * 4> h;
+#pragma unroll
+    for (int k = 0; k < K; ++k) z[k] = none ? 0.f : tile_hess(up, least, z[k]);
+    memcpy(&h, z, sizeof z);
+    h.store(a.out.hess + r * a.out.hess_stride);
+  }
 }
 
 // ---- launches ---------------------------------------------------------------
@@ -924,22 +1012,51 @@ u32 row_vectors(const Margins& m) {
 template <class T, TileMode kMode, int KT, int NT>
 void launch_tile_of(const TileArgs& t, cudaStream_t s) {
   const u64 K = t.row.m.classes, size = (NT * K * sizeof(T) + 15) / 16 * 16 + (t.row.out.hess ? NT * K * 4 : 0);
-  auto* const kernel = k_row_tile<T, kMode, KT, NT>;
-  if (size > 48 * 1024) DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(size)));
-  // lanes `spread` apart would meet in a bank: the row length's common factor with the banks
+  // lanes `spread` apart would meet in a bank: 32 by the row length's common factor with the banks
   const u32 words = u32(K * sizeof(T) % 4 ? 1 : K * sizeof(T) / 4);
   u32 spread = 32;
   while (spread > 1 && words % (64 / spread) == 0) spread /= 2;
+  auto* const kernel = spread <= 4 ? k_row_tile<T, kMode, KT, NT, true> : k_row_tile<T, kMode, KT, NT, false>;
+  if (size > 48 * 1024) DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(size)));
   kernel<<<grid_of((t.row.m.rows + NT - 1) / NT), NT, size, s>>>(t, spread);
+}
+// Whether every row of an array lies on the boundaries of its B bytes.
+inline bool on_boundaries(const void* p, u64 rows, u64 stride, u64 size, u64 B) {
+  const u64 unit = B < 16 ? B : 16;
+  return !p || (reinterpret_cast<std::uintptr_t>(p) % unit == 0 && (rows <= 1 || stride * size % unit == 0));
 }
 template <class T, TileMode kMode>
 void launch_tile(const TileArgs& t, cudaStream_t s) {
-  const u32 K = t.row.m.classes;
-  if (K <= 4) launch_tile_of<T, kMode, 4, 256>(t, s);
-  else if (K <= 8) launch_tile_of<T, kMode, 8, 256>(t, s);
-  else if (K <= 16) launch_tile_of<T, kMode, 16, 256>(t, s);
-  else if (K <= 32) launch_tile_of<T, kMode, 32, 128>(t, s);
-  else launch_tile_of<T, kMode, 64, 128>(t, s);
+  const RowArgs& a = t.row;
+  const u32 K = a.m.classes;
+  const u64 B = K * sizeof(T);
+  if ((B & (B - 1)) == 0 && B >= 4 && B <= 64 && K <= 16 && on_boundaries(a.m.z, a.m.rows, a.m.stride, sizeof(T), B) &&
+      on_boundaries(a.out.grad, a.m.rows, a.out.grad_stride, sizeof(T), B) &&
+      on_boundaries(a.out.hess, a.m.rows, a.out.hess_stride, 4, K * 4)) {
+    const u32 grid = grid_of((a.m.rows + 255) / 256);
+    if constexpr (sizeof(T) == 4)
+      if (K == 1) k_row_thread<T, kMode, 1><<<grid, 256, 0, s>>>(t);
+    if (K == 2) k_row_thread<T, kMode, 2><<<grid, 256, 0, s>>>(t);
+    if (K == 4) k_row_thread<T, kMode, 4><<<grid, 256, 0, s>>>(t);
+    if (K == 8) k_row_thread<T, kMode, 8><<<grid, 256, 0, s>>>(t);
+    if (K == 16) k_row_thread<T, kMode, 16><<<grid, 256, 0, s>>>(t);
+  } else if (K <= 4) {
+    launch_tile_of<T, kMode, 4, 256>(t, s);
+  } else if (K <= 8) {
+    launch_tile_of<T, kMode, 8, 256>(t, s);
+  } else if (K <= 12) {
+    launch_tile_of<T, kMode, 12, 256>(t, s);
+  } else if (K <= 16) {
+    launch_tile_of<T, kMode, 16, 256>(t, s);
+  } else if (K <= 24) {
+    launch_tile_of<T, kMode, 24, 128>(t, s);
+  } else if (K <= 32) {
+    launch_tile_of<T, kMode, 32, 128>(t, s);
+  } else if (K <= 48) {
+    launch_tile_of<T, kMode, 48, 128>(t, s);
+  } else {
+    launch_tile_of<T, kMode, 64, 128>(t, s);
+  }
 }
 
 template <class T, bool kPolicy, int G>
