@@ -1115,6 +1115,31 @@ inline u32 few_rows_cluster(u64 rows, u32 nvec, u32 blocks) {
   return blocks;
 }
 
+// Threads that share a row in the ring kernel.  The fewer, the less of the
+// time goes into joining their sums (134M bf16 margins in 16,384 rows: 46 us
+// by 32 threads, 50 by 64, 57 by 256; the forward and backward pass 107 by 64,
+// 124 by 256); but a row that is to stay for its gradient (`stays` vectors)
+// has to fit in their ring, and the rows should come out even over the places
+// that the device has (4096 rows over 3552 places of 32 threads leave most of
+// them idle for half of the time).
+inline u32 ring_threads(u64 rows, u32 stays) {
+  u32 best = 256;
+  double most = 0.0;
+  const double ease[4] = {1.0, 0.97, 0.93, 0.87};
+  for (int i = 0; i < 4; ++i) {
+    const u32 threads = 32u << i;
+    const u64 places = u64(kSMs) * (24 >> i);
+    if (threads < 256 && (stays > threads * 16 || rows * 2 < places)) continue;
+    const u64 rounds = (rows + places - 1) / places;
+    const double share = ease[i] * double(rows) / double(rounds * places);
+    if (share > most || threads == 256 && most == 0.0) {
+      most = share;
+      best = threads;
+    }
+  }
+  return best;
+}
+
 template <class T, bool kPolicy>
 void launch_rows_of(const RowArgs& a, cudaStream_t s) {
   if (!a.m.rows) return;
@@ -1126,30 +1151,18 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
     launch_lanes<T, kPolicy, 8>(a, (nvec + 7) / 8, s);
   } else if (nvec <= 32 * V) {
     launch_lanes<T, kPolicy, 32>(a, (nvec + 31) / 32, s);
-  } else if (!kPolicy) {
-    // Streaming: the fewer threads a row has, the less of the time goes into
-    // joining their sums, as long as the rows fill the device (134M bf16
-    // margins in rows of 8192: 46 us by 32 threads, 50 by 64, 57 by 256; of
-    // 131072, 1024 rows: 47 by 256 threads).
-    const u64 per_sm = a.m.rows / kSMs;
-    if (per_sm >= 24) launch_ring<T, kPolicy, 32, 4, 4, 24>(a, 1, s);
-    else if (per_sm >= 12) launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s);
-    else if (per_sm >= 6) launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s);
-    else launch_ring<T, kPolicy, 256, 4, 4, 3>(a, few_rows_cluster(a.m.rows, nvec, 1), s);
   } else {
-    // As few threads as have the ring for a row, on the same grounds; a row
-    // past the largest ring is cut over a cluster of blocks.
-    const u64 per_sm = a.m.rows / kSMs;
-    if (nvec <= 512 && per_sm >= 12) {
-      launch_ring<T, kPolicy, 32, 4, 4, 24>(a, 1, s);
-    } else if (nvec <= 1024 && per_sm >= 6) {
-      launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s);
-    } else if (nvec <= 2048 && per_sm >= 3) {
-      launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s);
-    } else {
-      u32 blocks = 1;
-      while (blocks < kMaxCluster && nvec > blocks * (256u * 4 * 4)) blocks *= 2;
-      launch_ring<T, kPolicy, 256, 4, 4, 3>(a, few_rows_cluster(a.m.rows, nvec, blocks), s);
+    // (whether a gradient is asked for changes nothing: the loss keeps its bits)
+    switch (ring_threads(a.m.rows, kPolicy ? nvec : 0)) {
+      case 32: launch_ring<T, kPolicy, 32, 4, 4, 24>(a, 1, s); break;
+      case 64: launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s); break;
+      case 128: launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s); break;
+      default: {
+        // a row past the ring is cut over a cluster of blocks
+        u32 blocks = 1;
+        while (kPolicy && blocks < kMaxCluster && nvec > blocks * (256u * 4 * 4)) blocks *= 2;
+        launch_ring<T, kPolicy, 256, 4, 4, 3>(a, few_rows_cluster(a.m.rows, nvec, blocks), s);
+      }
     }
   }
   after_launch("row loss");

@@ -147,6 +147,17 @@ def test_row_counts(dp, dtype, rows, classes):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,classes,pad", [(3600, 2051, 0), (1800, 4104, 3), (900, 8208, 0), (460, 16400, 1)])
+def test_many_long_rows(dp, dtype, rows, classes, pad):
+    """As many rows as fill the device with 32, 64 and 128 threads a row, runs
+    of skipped rows among them."""
+    z, z64, rng = margins(rows, classes, dtype, rows + pad, pad, pad)
+    y = labels(rng, rows, classes)
+    y[rows // 3: rows // 2] = -1
+    check_rows(dp, z, z64, y, rng, dtype, hess=False, in_place=pad > 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("classes", [5, 33, 129, 1001, 9000, 70001])
 def test_gradient_in_the_margins_place(dp, dtype, classes):
     for pad, shift in ((0, 0), (5, 2)):
