@@ -789,7 +789,7 @@ struct TileArgs {
   const float* weight;   // and the loss's derivatives
 };
 enum TileMode { kTileLogProb, kTilePolicy, kTileGrad };
-constexpr u32 kTileClasses = 64;
+constexpr u32 kTileClasses = 64;  // the most that its registers hold
 
 // Copies `rows` rows of K elements between memory (`stride` apart) and a tile
 // without gaps; whole vectors when the rows have no gaps either.
@@ -1059,6 +1059,16 @@ void launch_tile(const TileArgs& t, cudaStream_t s) {
   }
 }
 
+// One thread a row up to 16 classes; up to 64 also where rows lie off the
+// 16-byte boundaries, which lanes would take element by element at both ends
+// (67M margins, lanes and tile: 64 bf16 classes 61 and 131 us, 33 145 and 104;
+// fp32 104 and 145, 150 and 127).
+template <class T>
+bool use_tile(const Margins& m) {
+  return m.classes <= 16 || (m.classes <= kTileClasses &&
+                             !(m.classes * sizeof(T) % 16 == 0 && on_boundaries(m.z, m.rows, m.stride, sizeof(T), 16)));
+}
+
 template <class T, bool kPolicy, int G>
 void launch_lanes(const RowArgs& a, u32 per_lane, cudaStream_t s) {
   const u32 grid = grid_of((a.m.rows + 256 / G - 1) / (256 / G));
@@ -1116,23 +1126,21 @@ inline u32 few_rows_cluster(u64 rows, u32 nvec, u32 blocks) {
 }
 
 // Threads that share a row in the ring kernel.  The fewer, the less of the
-// time goes into joining their sums (134M bf16 margins in 16,384 rows: 46 us
-// by 32 threads, 50 by 64, 57 by 256; the forward and backward pass 107 by 64,
-// 124 by 256); but a row that is to stay for its gradient (`stays` vectors)
-// has to fit in their ring, and the rows should come out even over the places
-// that the device has (4096 rows over 3552 places of 32 threads leave most of
-// them idle for half of the time).
-inline u32 ring_threads(u64 rows, u32 stays) {
+// time goes into joining their sums: about what three and a half vectors a
+// thread take (134M bf16 margins in 16,384 rows: 46 us by 32 threads, 50 by
+// 64, 55 by 128, 57 by 256).  But a row that is to stay for its gradient
+// (`stays`) has to fit in their ring, 16 vectors a thread, and the rows should
+// come out even over the places that the device has for them (4096 rows over
+// 3552 places of 32 threads would leave most idle for half of the time).
+inline u32 ring_threads(u64 rows, u32 nvec, bool stays) {
   u32 best = 256;
   double most = 0.0;
-  const double ease[4] = {1.0, 0.97, 0.93, 0.87};
-  for (int i = 0; i < 4; ++i) {
-    const u32 threads = 32u << i;
-    const u64 places = u64(kSMs) * (24 >> i);
-    if (threads < 256 && (stays > threads * 16 || rows * 2 < places)) continue;
-    const u64 rounds = (rows + places - 1) / places;
-    const double share = ease[i] * double(rows) / double(rounds * places);
-    if (share > most || threads == 256 && most == 0.0) {
+  for (u32 threads = 32; threads <= 256; threads *= 2) {
+    const u64 places = u64(kSMs) * 24 * 32 / threads;
+    if (threads < 256 && ((stays && nvec > threads * 16) || rows * 2 < places)) continue;
+    const double each = double(nvec) / threads;
+    const double share = each / (each + 3.5) * double(rows) / double((rows + places - 1) / places * places);
+    if (share > most) {
       most = share;
       best = threads;
     }
@@ -1144,16 +1152,26 @@ template <class T, bool kPolicy>
 void launch_rows_of(const RowArgs& a, cudaStream_t s) {
   if (!a.m.rows) return;
   constexpr u32 V = 8;  // most vectors a lane holds
-  const u32 K = a.m.classes, nvec = row_vectors<T>(a.m);
-  if (K <= kTileClasses) {
+  const u32 nvec = row_vectors<T>(a.m);
+  if (use_tile<T>(a.m)) {
     launch_tile<T, kPolicy ? kTilePolicy : kTileLogProb>(TileArgs{a, nullptr, nullptr}, s);
+  } else if (nvec <= 2 * V) {
+    // As few lanes as hold the row with up to eight vectors each, for a row's
+    // scalars are every lane's work (67M bf16 margins, with up to eight and up
+    // to four: rows of 80 56 and 75 us, of 128 63 and 57, of 256 54 and 55, of
+    // 300 63 and 84).
+    launch_lanes<T, kPolicy, 2>(a, (nvec + 1) / 2, s);
+  } else if (nvec <= 4 * V) {
+    launch_lanes<T, kPolicy, 4>(a, (nvec + 3) / 4, s);
   } else if (nvec <= 8 * V) {
     launch_lanes<T, kPolicy, 8>(a, (nvec + 7) / 8, s);
+  } else if (nvec <= 16 * V) {
+    launch_lanes<T, kPolicy, 16>(a, (nvec + 15) / 16, s);
   } else if (nvec <= 32 * V) {
     launch_lanes<T, kPolicy, 32>(a, (nvec + 31) / 32, s);
   } else {
     // (whether a gradient is asked for changes nothing: the loss keeps its bits)
-    switch (ring_threads(a.m.rows, kPolicy ? nvec : 0)) {
+    switch (ring_threads(a.m.rows, nvec, kPolicy)) {
       case 32: launch_ring<T, kPolicy, 32, 4, 4, 24>(a, 1, s); break;
       case 64: launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s); break;
       case 128: launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s); break;
@@ -1168,26 +1186,36 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
   after_launch("row loss");
 }
 
+// G threads a piece of a row, U vectors each.
+template <class T, int G>
+void launch_grad_pieces(const GradArgs& a, u32 nvec, cudaStream_t s) {
+  constexpr u32 U = 4, per_block = 256 / G;
+  const u32 pieces = (nvec + G * U - 1) / (G * U);
+  k_log_prob_grad<T, G, U><<<grid_of((a.m.rows * pieces + per_block - 1) / per_block), 256, 0, s>>>(a, pieces);
+}
+
 template <class T>
 void launch_grad_of(const GradArgs& a, cudaStream_t s) {
   if (!a.m.rows) return;
-  const u64 rows = a.m.rows;
   const u32 nvec = row_vectors<T>(a.m);
-  constexpr u32 U = 4;
-  if (a.m.classes <= kTileClasses) {
+  if (use_tile<T>(a.m)) {
     RowArgs row{};
     row.m = a.m;
     row.label = a.label;
     row.out = a.out;
     launch_tile<T, kTileGrad>(TileArgs{row, a.norm, a.weight}, s);
-  } else if (nvec <= 8 * U) {
-    k_log_prob_grad<T, 8, U><<<grid_of((rows + 31) / 32), 256, 0, s>>>(a, 1u);
-  } else if (nvec <= 32 * U * 2) {
-    const u32 pieces = (nvec + 32 * U - 1) / (32 * U);
-    k_log_prob_grad<T, 32, U><<<grid_of((rows * pieces + 7) / 8), 256, 0, s>>>(a, pieces);
+  } else if (nvec <= 8) {
+    launch_grad_pieces<T, 2>(a, nvec, s);
+  } else if (nvec <= 16) {
+    launch_grad_pieces<T, 4>(a, nvec, s);
+  } else if (nvec <= 32) {
+    launch_grad_pieces<T, 8>(a, nvec, s);
+  } else if (nvec <= 64) {
+    launch_grad_pieces<T, 16>(a, nvec, s);
+  } else if (nvec <= 1024) {
+    launch_grad_pieces<T, 32>(a, nvec, s);
   } else {
-    const u32 pieces = (nvec + 256 * U - 1) / (256 * U);
-    k_log_prob_grad<T, 256, U><<<grid_of(rows * pieces), 256, 0, s>>>(a, pieces);
+    launch_grad_pieces<T, 256>(a, nvec, s);
   }
   after_launch("log_prob_grad");
 }
