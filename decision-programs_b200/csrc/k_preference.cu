@@ -72,15 +72,24 @@ __device__ __forceinline__ float lanes_sum(float v) {
   for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+template <int U>
 __device__ __forceinline__ float span_sum(const PairLoss& a, u64 b, u64 e, u64 first, u64 step) {
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  u64 r = b + first;
-  for (; r + 3 * step < e; r += 4 * step) {
+  float s[U], v[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] += gap(a, r + i * step);
+  for (int i = 0; i < U; ++i) s[i] = 0.f;
+  u64 r = b + first;
+  for (; r + (U - 1) * step < e; r += U * step) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) v[i] = gap(a, r + i * step);
+#pragma unroll
+    for (int i = 0; i < U; ++i) s[i] += v[i];
   }
   for (; r < e; r += step) s[0] += gap(a, r);
-  return (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int d = U / 2; d > 0; d /= 2)
+#pragma unroll
+    for (int i = 0; i < d; ++i) s[i] += s[i + d];
+  return s[0];
 }
 __device__ __forceinline__ void span_fill(const PairLoss& a, u64 b, u64 e, u64 first, u64 step, float q, float h) {
 #pragma unroll 4
@@ -100,6 +109,56 @@ __device__ __forceinline__ void fill_outside(const PairLoss& a, u64 rows, const 
   span_fill(a, last, rows, me, step, 0.f, item_hess(0.f));
 }
 
+// Items of a few rows: a block stages the rows of 256 pairs in shared memory,
+// a thread takes a pair, and the gradients go out as the scores came in, in
+// whole lines.  (4M rows in 1M pairs: 118 us by 8 lanes a pair.)  Blocks whose
+// rows do not fit take their pairs one thread each from memory.
+constexpr u32 kPairBlock = 256, kStageRows = 4096;
+__global__ void __launch_bounds__(kPairBlock) k_preference_staged(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
+  __shared__ float stage[kStageRows];
+  __shared__ float stage_h[kStageRows];
+  const u64 p0 = u64(blockIdx.x) * kPairBlock, p1 = min(pairs, p0 + kPairBlock), p = p0 + threadIdx.x;
+  const u64 r0 = clamp_row(begin[2 * p0], rows), r1 = clamp_row(begin[2 * p1], rows);
+  const bool in = p < p1;
+  const u64 b0 = in ? clamp_row(begin[2 * p], rows) : 0, b1 = in ? clamp_row(begin[2 * p + 1], rows) : 0,
+            b2 = in ? clamp_row(begin[2 * p + 2], rows) : 0;
+  const float w = in && a.weight ? a.weight[p] : 1.f;
+  const bool fits = r1 >= r0 && r1 - r0 <= kStageRows;
+  const u32 n = fits ? u32(r1 - r0) : 0;
+  for (u32 i = threadIdx.x; i < n; i += kPairBlock) stage[i] = gap(a, r0 + i);
+  __syncthreads();
+  // (offsets out of order lead outside a pair's own rows, not outside the stage)
+  auto local = [&](u64 b) { return b <= r0 ? 0u : u32(min(u64(n), b - r0)); };
+  const u32 c0 = local(b0), c1 = local(b1), c2 = local(b2);
+  float sa = 0.f, sb = 0.f;
+  if (fits) {
+    for (u32 i = c0; i < c1; ++i) sa += stage[i];
+    for (u32 i = c1; i < c2; ++i) sb += stage[i];
+  } else {
+    sa = span_sum<4>(a, b0, b1, 0, 1);
+    sb = span_sum<4>(a, b1, b2, 0, 1);
+  }
+  const PairResult o = pair_result(a, sa - sb, w);
+  const float h = item_hess(o.h);
+  if (in) a.loss[p] = o.loss;
+  if (fits) {
+    __syncthreads();  // (every sum has been taken)
+    if (in) {
+      for (u32 i = c0; i < c1; ++i) { stage[i] = o.q; stage_h[i] = h; }
+      for (u32 i = c1; i < c2; ++i) { stage[i] = -o.q; stage_h[i] = h; }
+    }
+    __syncthreads();
+    for (u32 i = threadIdx.x; i < n; i += kPairBlock) {
+      a.grad[r0 + i] = stage[i];
+      if (a.hess) a.hess[r0 + i] = stage_h[i];
+    }
+  } else if (in) {
+    span_fill(a, b0, b1, 0, 1, o.q, h);
+    span_fill(a, b1, b2, 0, 1, -o.q, h);
+  }
+  fill_outside(a, rows, begin, pairs);
+}
+
 // Short items: G lanes a pair.
 template <int G>
 __global__ void __launch_bounds__(256) k_preference_lanes(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
@@ -110,7 +169,7 @@ __global__ void __launch_bounds__(256) k_preference_lanes(PairLoss a, u64 rows, 
     const bool in = p < pairs;  // (the lanes of a warp sum together)
     const u64 b0 = in ? clamp_row(begin[2 * p], rows) : 0, b1 = in ? clamp_row(begin[2 * p + 1], rows) : 0,
               b2 = in ? clamp_row(begin[2 * p + 2], rows) : 0;
-    const float sa = lanes_sum<G>(span_sum(a, b0, b1, lane, G)), sb = lanes_sum<G>(span_sum(a, b1, b2, lane, G));
+    const float sa = lanes_sum<G>(span_sum<4>(a, b0, b1, lane, G)), sb = lanes_sum<G>(span_sum<4>(a, b1, b2, lane, G));
     if (!in) continue;
     const PairResult o = pair_result(a, sa - sb, a.weight ? a.weight[p] : 1.f);
     const float h = item_hess(o.h);
@@ -123,21 +182,22 @@ __global__ void __launch_bounds__(256) k_preference_lanes(PairLoss a, u64 rows, 
 
 // Long items: a block, or a cluster of blocks, a pair.
 constexpr u32 kPairCluster = 8;
-__global__ void __launch_bounds__(512) k_preference_block(PairLoss a, u64 rows, const i64* begin, u64 pairs, u32 blocks) {
-  constexpr u32 kWarps = 512 / 32;
+template <int kBlockThreads, int U>
+__global__ void __launch_bounds__(kBlockThreads) k_preference_block(PairLoss a, u64 rows, const i64* begin, u64 pairs, u32 blocks) {
+  constexpr u32 kWarps = kBlockThreads / 32;
   __shared__ float2 part[2][kWarps], blocks_part[2][kPairCluster];
   u32 rank = 0, parity = 0;
   if (blocks > 1) {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
-  const u64 first = rank * 512 + threadIdx.x, step = u64(blocks) * 512;
+  const u64 first = rank * kBlockThreads + threadIdx.x, step = u64(blocks) * kBlockThreads;
   for (u64 p = blockIdx.x / blocks; p < pairs; p += gridDim.x / blocks) {
     const u64 b0 = clamp_row(begin[2 * p], rows), b1 = clamp_row(begin[2 * p + 1], rows),
               b2 = clamp_row(begin[2 * p + 2], rows);
     float2 s;
-    s.x = lanes_sum<32>(span_sum(a, b0, b1, first, step));
-    s.y = lanes_sum<32>(span_sum(a, b1, b2, first, step));
+    s.x = lanes_sum<32>(span_sum<U>(a, b0, b1, first, step));
+    s.y = lanes_sum<32>(span_sum<U>(a, b1, b2, first, step));
     if ((threadIdx.x & 31) == 0) part[parity][threadIdx.x >> 5] = s;
     __syncthreads();
     s = part[parity][threadIdx.x & (kWarps - 1)];
@@ -466,18 +526,24 @@ void launch_preference(const PairLoss& a, u64 rows, const i64* begin, u64 pairs,
       k_preference_rows<false><<<blocks_for(rows / 2 + 1, 256), 256, 0, s>>>(a, rows, pairs);
     else
       k_preference_rows<true><<<blocks_for(rows / 2 + 1, 256), 256, 0, s>>>(a, rows, pairs);
+  } else if (average <= 12 && pairs >= 1024) {
+    need(pairs <= (u64(kPairBlock) << 31), "too many pairs for one launch");
+    k_preference_staged<<<u32((pairs + kPairBlock - 1) / kPairBlock), kPairBlock, 0, s>>>(a, rows, begin, pairs);
   } else if (average < 64 && pairs >= 64) {
     k_preference_lanes<8><<<blocks_for(pairs, 32), 256, 0, s>>>(a, rows, begin, pairs);
   } else if (average < 1024 && pairs >= 4 * kSMs) {
     k_preference_lanes<32><<<blocks_for(pairs, 8), 256, 0, s>>>(a, rows, begin, pairs);
   } else {
-    // a block a pair; few pairs of very many rows: a cluster of blocks each
+    // A block a pair; few pairs of very many rows: a cluster of larger blocks
+    // each, with more loads under way (one pair of 4M rows: 184 us by eight
+    // blocks of 512 threads, 84 by eight of 1024; 1000 pairs of 4000: 19 and 41).
     u32 blocks = 1;
     while (blocks < kPairCluster && pairs * blocks * 2 <= kSMs && average > 4096u * blocks) blocks *= 2;
-    const u64 clusters = pairs < 1 ? 1 : (pairs < kSMs * 4 ? pairs : kSMs * 4);
+    const bool large = average >= 32768;
+    const u64 most = kSMs * (large ? 2 : 4), clusters = pairs < 1 ? 1 : (pairs < most ? pairs : most);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(u32(clusters * blocks));
-    cfg.blockDim = dim3(512);
+    cfg.blockDim = dim3(large ? 1024 : 512);
     cfg.stream = s;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -485,7 +551,8 @@ void launch_preference(const PairLoss& a, u64 rows, const i64* begin, u64 pairs,
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = blocks > 1 ? 1 : 0;
-    DP_CUDA((cudaLaunchKernelEx(&cfg, k_preference_block, a, rows, begin, pairs, blocks)));
+    auto* const kernel = large ? k_preference_block<1024, 8> : k_preference_block<512, 4>;
+    DP_CUDA((cudaLaunchKernelEx(&cfg, kernel, a, rows, begin, pairs, blocks)));
   }
   after_launch("preference loss");
 }

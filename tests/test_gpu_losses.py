@@ -338,11 +338,12 @@ def pair_bound(x, terms, w, beta, x_err):
 
 @pytest.mark.parametrize("use_ref", [False, True])
 @pytest.mark.parametrize("smoothing", [0.0, 0.1])
-@pytest.mark.parametrize("lengths", ["one", "short", "mixed", "long", "empty", "huge"])
+@pytest.mark.parametrize("lengths", ["one", "short", "few", "uneven", "mixed", "long", "empty", "huge"])
 def test_preference_over_segments(dp, lengths, smoothing, use_ref):
     rng = np.random.default_rng(7)
-    items = {"one": 4000, "short": 600, "mixed": 200, "long": 6, "empty": 50, "huge": 2}[lengths]
-    n = {"one": np.ones(items, int), "short": rng.integers(1, 9, items), "mixed": rng.integers(0, 700, items),
+    items = {"one": 4000, "short": 600, "few": 9000, "uneven": 5000, "mixed": 200, "long": 6, "empty": 50, "huge": 2}[lengths]
+    n = {"one": np.ones(items, int), "short": rng.integers(1, 9, items), "few": rng.integers(0, 9, items),
+         "uneven": np.where(rng.random(items) < 0.002, 3000, rng.integers(0, 4, items)), "mixed": rng.integers(0, 700, items),
          "long": rng.integers(3000, 9000, items), "empty": rng.integers(0, 2, items),
          "huge": np.array([300_001, 77_777])}[lengths]
     lead, tail = (0, 0) if lengths == "one" else (3, 5)
