@@ -42,13 +42,21 @@ Span span_of(const void* p, u64 rows, u64 width, u64 stride, u64 size) {
 }
 bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
 
+// A check whose message names an argument; it is put together only on failure.
+void need_of(bool ok, const char* what, const char* rule) {
+  if (!ok) dp::fail(std::string(what) + " " + rule);
+}
 void check_rows(u64 rows, u64 width, u64 stride, u64 size, const void* p, const char* what) {
-  const std::string w(what);
-  need(stride >= width, w + " row stride must cover the classes");
-  need(stride <= (u64(1) << 40), w + " row stride out of range");
-  need(rows <= (u64(1) << 62) / 8 / (stride ? stride : 1), w + " size overflows 64-bit byte offsets");
-  need(rows == 0 || p != nullptr, w + " pointer is null");
-  need(reinterpret_cast<std::uintptr_t>(p) % size == 0, w + " pointer is not aligned to its type");
+  need_of(stride >= width, what, "row stride must cover the classes");
+  need_of(stride <= (u64(1) << 40), what, "row stride out of range");
+  need_of(rows <= (u64(1) << 62) / 8 / (stride ? stride : 1), what, "size overflows 64-bit byte offsets");
+  need_of(rows == 0 || p != nullptr, what, "pointer is null");
+  need_of(reinterpret_cast<std::uintptr_t>(p) % size == 0, what, "pointer is not aligned to its type");
+}
+// Vectors: an address off its type's boundary would fault on the device.
+template <class... P>
+void check_aligned(const P*... p) {
+  need(((reinterpret_cast<std::uintptr_t>(p) % sizeof(P) == 0) && ...), "a vector's pointer is not aligned to its type");
 }
 
 dp::Margins margins_of(int32_t dtype, const void* margin, u64 rows, uint32_t classes, u64 stride) {
@@ -88,6 +96,7 @@ dp::PairLoss pair_args(const float* score, const float* ref, const float* weight
   need(smoothing >= 0.f && smoothing <= 0.5f, "label smoothing must be in [0, 0.5]");
   need(rows == 0 || (score != nullptr && grad != nullptr), "score or gradient pointer is null");
   need(pairs == 0 || loss != nullptr, "loss pointer is null");
+  check_aligned(score, ref, weight, loss, grad, hess);
   dp::PairLoss a{};
   a.score = score;
   a.ref = ref;
@@ -111,6 +120,7 @@ int dp_log_prob(int32_t dtype, const void* margin, uint64_t rows, uint32_t class
     need(rows == 0 || (label != nullptr && log_prob != nullptr && norm != nullptr),
          "label, log-probability or norm pointer is null");
     need(reinterpret_cast<std::uintptr_t>(norm) % sizeof(float2) == 0, "norm pointer is not aligned to 8 bytes");
+    check_aligned(label, log_prob);
     dp::RowArgs a{};
     a.m = m;
     a.label = label;
@@ -128,6 +138,7 @@ int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, uint32_t 
     need(rows == 0 || (label != nullptr && norm != nullptr && weight != nullptr && grad != nullptr),
          "label, norm, weight or gradient pointer is null");
     need(reinterpret_cast<std::uintptr_t>(norm) % sizeof(float2) == 0, "norm pointer is not aligned to 8 bytes");
+    check_aligned(label, weight);
     const dp::MarginGrad g = grad_of(m, grad, grad_stride, hess, hess_stride);
     dp::launch_grad(dp::GradArgs{m, label, reinterpret_cast<const float2*>(norm), weight, g},
                     static_cast<cudaStream_t>(stream));
@@ -144,6 +155,7 @@ int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t cl
     need(rows == 0 || (label != nullptr && old_log_prob != nullptr && advantage != nullptr),
          "label, old log-probability or advantage pointer is null");
     need(rows == 0 || (loss != nullptr && log_prob != nullptr), "loss or log-probability pointer is null");
+    check_aligned(label, old_log_prob, ref_log_prob, advantage, weight, loss, log_prob);
     need(clip_low >= 0.f && clip_low <= 1.f, "clip_low must be in [0, 1]");
     need(std::isfinite(clip_high) && clip_high >= 0.f, "clip_high must be finite and not negative");
     need(std::isfinite(kl) && kl >= 0.f, "the KL coefficient must be finite and not negative");
@@ -170,6 +182,7 @@ int dp_preference_loss(uint64_t rows, const int64_t* item_begin, uint64_t pairs,
                        float* grad, float* hess, void* stream) {
   return guarded([&] {
     need(rows < (u64(1) << 60) && pairs < (u64(1) << 40), "rows or pairs out of range");
+    check_aligned(item_begin);
     need(item_begin != nullptr || rows >= 2 * pairs, "without item offsets every pair needs two rows");
     const dp::PairLoss a =
         pair_args(score, ref_score, weight, beta, smoothing, loss, grad, hess, rows, pairs);
@@ -182,6 +195,7 @@ int dp_preference_prepare(uint64_t rows, const int32_t* pair_rows, uint64_t pair
     need(out_plan != nullptr, "output pointer is null");
     need(rows < (u64(1) << 31) && pairs < (u64(1) << 31), "rows and pairs must be below 2^31");
     need(pairs == 0 || pair_rows != nullptr, "pair pointer is null");
+    check_aligned(pair_rows);
     auto plan = std::make_unique<dp::PairPlan>();
     dp::build_pair_plan(*plan, rows, pair_rows, pairs, static_cast<cudaStream_t>(stream));
     *out_plan = plan.release();

@@ -364,9 +364,15 @@ constexpr u32 kMaxCluster = 8;
 // The maximum and the sum over the blocks of a cluster, in the order of their
 // ranks: every block gets the same two numbers.
 __device__ __forceinline__ void cluster_join(float2* parts, u32 blocks, float& m, float& s) {
-  if (threadIdx.x < blocks) cluster_put(parts + cluster_rank(), threadIdx.x, make_float2(m, s));
-  __syncwarp();
-  cluster_arrive();
+  // Only the warp that has written to the other blocks arrives with release:
+  // it would make the others wait for their last row's gradients to arrive.
+  if (threadIdx.x < 32) {
+    if (threadIdx.x < blocks) cluster_put(parts + cluster_rank(), threadIdx.x, make_float2(m, s));
+    __syncwarp();
+    cluster_arrive();
+  } else {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  }
   cluster_wait();
   float top = neg_inf();
   for (u32 b = 0; b < blocks; ++b) top = fmaxf(top, parts[b].x);

@@ -304,8 +304,8 @@ DP_API int dp_eval_splits(const int64_t* hist, int32_t nnodes, uint32_t features
  * margin: [rows][classes] of `dtype` 0 fp32, 1 fp16 or 2 bf16, rows
  * `row_stride` elements apart, any alignment of the type.  Sums and
  * exponentials are fp32; a gradient is rounded to `dtype` once.
- *  - label (int32) outside [0, classes): the row is skipped: its margins are
- *    not read, its outputs and its gradient row are 0.
+ *  - label (int32) outside [0, classes): the row is skipped: whatever its
+ *    margins hold, its outputs and its gradient row are 0.
  *  - margins of -inf are masked classes of probability 0.  A row that masks
  *    every class has log-probability -inf, loss 0 and a zero gradient.
  *  - NaN or +inf in a row that is not skipped makes that row's results NaN,
@@ -318,8 +318,8 @@ DP_API int dp_log_prob(int32_t dtype, const void* margin, uint64_t rows, uint32_
 /* The backward pass: grad[rows][classes] (of `dtype`) = weight[r] *
  * ([k == label] - p_k), weight being the derivative of a loss by log_prob[r];
  * hess (fp32, may be NULL) = |weight[r]| * max(2 p_k (1 - p_k), 1e-16), the
- * softmax objective's diagonal form.  weight 0: the row's margins are not read
- * and its outputs are 0.  grad may be margin itself (same row stride);
+ * softmax objective's diagonal form.  weight 0: the row's outputs are 0,
+ * whatever its margins hold.  grad may be margin itself (same row stride);
  * other overlaps are refused. */
 DP_API int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
                             const int32_t* label, const float* norm, const float* weight, void* grad,

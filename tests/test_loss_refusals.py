@@ -73,6 +73,20 @@ def test_preference_checks(dp):
     assert dp.lib().dp_preference_free(None) == 0
 
 
+def test_vectors_off_their_boundaries(dp):
+    odd = A + 2
+    lead = (0, A, 4, 10, 10)
+    for label, out in ((odd, A), (A, odd)):
+        assert "not aligned" in refused(dp, "dp_log_prob", *lead, label, out, A, None)
+    assert "not aligned" in refused(dp, "dp_log_prob_grad", *lead, A, A, odd, 1 << 20, 10, None, 0, None)
+    assert "not aligned" in refused(dp, "dp_policy_loss", *lead, A, A, None, odd, None, 0.2, 0.2, 0.0, A, A, None, 0,
+                                    None, 0, None)
+    assert "not aligned" in refused(dp, "dp_preference_loss", 8, None, 4, odd, None, None, 1.0, 0.0, A, A, None, None)
+    assert "not aligned" in refused(dp, "dp_preference_loss", 8, A + 4, 4, A, None, None, 1.0, 0.0, A, A, None, None)
+    plan = C.c_void_p()
+    assert "not aligned" in refused(dp, "dp_preference_prepare", 4, odd, 4, None, C.byref(plan))
+
+
 def test_no_rows_need_no_device(dp):
     assert dp.lib().dp_log_prob(0, None, 0, 10, 10, None, None, None, None) == 0
     assert dp.lib().dp_log_prob_grad(2, None, 0, 10, 10, None, None, None, None, 10, None, 0, None) == 0
