@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(256, 4) k_row_loss(RowArgs a) {
     if (c == 0.f) {
       for (u32 j = cut.j0 + lane; j < cut.j1; j += G) out.zero(j);
     } else {
-      constexpr int U = V < 4 ? V : (V == 6 ? 3 : 4);
+      constexpr int U = V == 6 ? 3 : (V == 8 ? 4 : V);  // (V is a multiple of it)
 #pragma unroll
       for (int i = 0; i < V; i += U) {
         uint4 w[U];
@@ -1022,7 +1022,9 @@ void launch_tile_of(const TileArgs& t, cudaStream_t s) {
   const u32 words = u32(K * sizeof(T) % 4 ? 1 : K * sizeof(T) / 4);
   u32 spread = 32;
   while (spread > 1 && words % (64 / spread) == 0) spread /= 2;
-  auto* const kernel = spread <= 4 ? k_row_tile<T, kMode, KT, NT, true> : k_row_tile<T, kMode, KT, NT, false>;
+  auto* kernel = k_row_tile<T, kMode, KT, NT, false>;
+  if constexpr (KT % 8 == 0 && KT * sizeof(T) >= 32)
+    if (spread <= 4) kernel = k_row_tile<T, kMode, KT, NT, true>;
   if (size > 48 * 1024) DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(size)));
   kernel<<<grid_of((t.row.m.rows + NT - 1) / NT), NT, size, s>>>(t, spread);
 }
@@ -1075,15 +1077,20 @@ bool use_tile(const Margins& m) {
                              !(m.classes * sizeof(T) % 16 == 0 && on_boundaries(m.z, m.rows, m.stride, sizeof(T), 16)));
 }
 
+// (fewer vectors a lane are the next smaller G's)
 template <class T, bool kPolicy, int G>
-void launch_lanes(const RowArgs& a, u32 per_lane, cudaStream_t s) {
-  const u32 grid = grid_of((a.m.rows + 256 / G - 1) / (256 / G));
-  if (per_lane <= 1) k_row_loss<T, kPolicy, G, 1><<<grid, 256, 0, s>>>(a);
-  else if (per_lane <= 2) k_row_loss<T, kPolicy, G, 2><<<grid, 256, 0, s>>>(a);
-  else if (per_lane <= 3) k_row_loss<T, kPolicy, G, 3><<<grid, 256, 0, s>>>(a);
-  else if (per_lane <= 4) k_row_loss<T, kPolicy, G, 4><<<grid, 256, 0, s>>>(a);
-  else if (per_lane <= 6) k_row_loss<T, kPolicy, G, 6><<<grid, 256, 0, s>>>(a);
-  else k_row_loss<T, kPolicy, G, 8><<<grid, 256, 0, s>>>(a);
+void launch_lanes(const RowArgs& a, u32 nvec, cudaStream_t s) {
+  const u32 grid = grid_of((a.m.rows + 256 / G - 1) / (256 / G)), per_lane = (nvec + G - 1) / G;
+  if constexpr (G == 2) {
+    if (per_lane <= 2) k_row_loss<T, kPolicy, G, 2><<<grid, 256, 0, s>>>(a);
+    else if (per_lane <= 3) k_row_loss<T, kPolicy, G, 3><<<grid, 256, 0, s>>>(a);
+    else if (per_lane <= 4) k_row_loss<T, kPolicy, G, 4><<<grid, 256, 0, s>>>(a);
+  }
+  if (G > 2 || per_lane > 4) {
+    if (per_lane <= 5) k_row_loss<T, kPolicy, G, 5><<<grid, 256, 0, s>>>(a);
+    else if (per_lane <= 6) k_row_loss<T, kPolicy, G, 6><<<grid, 256, 0, s>>>(a);
+    else k_row_loss<T, kPolicy, G, 8><<<grid, 256, 0, s>>>(a);
+  }
 }
 
 template <class T, bool kPolicy, int NT, int U, int S, int kPerSM>
@@ -1166,15 +1173,15 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
     // scalars are every lane's work (67M bf16 margins, with up to eight and up
     // to four: rows of 80 56 and 75 us, of 128 63 and 57, of 256 54 and 55, of
     // 300 63 and 84).
-    launch_lanes<T, kPolicy, 2>(a, (nvec + 1) / 2, s);
+    launch_lanes<T, kPolicy, 2>(a, nvec, s);
   } else if (nvec <= 4 * V) {
-    launch_lanes<T, kPolicy, 4>(a, (nvec + 3) / 4, s);
+    launch_lanes<T, kPolicy, 4>(a, nvec, s);
   } else if (nvec <= 8 * V) {
-    launch_lanes<T, kPolicy, 8>(a, (nvec + 7) / 8, s);
+    launch_lanes<T, kPolicy, 8>(a, nvec, s);
   } else if (nvec <= 16 * V) {
-    launch_lanes<T, kPolicy, 16>(a, (nvec + 15) / 16, s);
+    launch_lanes<T, kPolicy, 16>(a, nvec, s);
   } else if (nvec <= 32 * V) {
-    launch_lanes<T, kPolicy, 32>(a, (nvec + 31) / 32, s);
+    launch_lanes<T, kPolicy, 32>(a, nvec, s);
   } else {
     // (whether a gradient is asked for changes nothing: the loss keeps its bits)
     switch (ring_threads(a.m.rows, nvec, kPolicy)) {
