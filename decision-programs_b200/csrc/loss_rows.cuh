@@ -12,7 +12,6 @@
 // such, the few elements before the first and after the last one by one, so
 // that nothing outside the row is read or written.
 #pragma once
-#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -474,14 +473,17 @@ __global__ void __launch_bounds__(256, 4) k_row_loss(RowArgs a) {
 }
 
 // ---- long rows --------------------------------------------------------------
-// `blocks` blocks of a cluster share a row, and each cluster walks its rows
-// (r, r + clusters, ...).  Every thread streams its own vectors through its
-// own places of a ring in shared memory, by asynchronous copies that run
-// ahead of it into the following rows, so that margins keep arriving while
-// sums are joined and gradients are written; nothing in the ring is shared,
-// so it needs no barrier.  A row that fits in the ring stays there between
-// its sum and its gradient (one read of the margins); a longer one is
-// streamed twice.
+// A block, or a cluster of `blocks` blocks, a row.  Every thread streams its
+// own vectors through its own places of a ring in shared memory, by
+// asynchronous copies that run ahead of it; nothing in the ring is shared, so
+// it needs no barrier.  A row that fits in the rings stays there between its
+// sum and its gradient (one read of the margins); a longer one is streamed
+// twice, the second time mostly from L2.  Blocks come and go with their rows:
+// several on an SM, in different places of theirs, keep memory and arithmetic
+// busy, and rows without a label, which cost half of the others or less, do
+// not leave some blocks with more work than others (8192 x 65,536 bf16, a
+// quarter without a label: 339 us; by resident blocks that take every n-th row
+// and copy ahead into the next one 448).
 __device__ __forceinline__ void copy_async(u32 shared, const void* global) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
 }
@@ -495,59 +497,6 @@ __device__ __forceinline__ void copy_wait(u32 n) {
   } else {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-}
-
-// The rows of one cluster in order, their labels read 32 at a time by each
-// warp for itself: what the copies run ahead by.
-struct RowWalk {
-  const i32* label;
-  u64 rows, step, r;
-  u32 at = 32;
-  i32 batch = -1;
-  __device__ __forceinline__ RowWalk(const RowArgs& a, u64 first, u64 clusters)
-      : label(a.label), rows(a.m.rows), step(clusters), r(first) {}
-  __device__ __forceinline__ bool done() const { return r >= rows; }
-  __device__ __forceinline__ i32 load() const {
-    const u64 mine = r + (threadIdx.x & 31) * step;
-    return mine < rows ? label[mine] : -1;
-  }
-  __device__ __forceinline__ i32 here() {
-    if (at == 32) {
-      batch = load();
-      at = 0;
-    }
-    return __shfl_sync(0xffffffffu, batch, at);
-  }
-  __device__ __forceinline__ void next() {
-    r += step;
-    ++at;
-  }
-};
-// The labels that a cluster goes by.  Whether a row takes part decides which
-// barriers its threads meet at, so one warp reads it for all of them: were the
-// labels written while the kernel runs, the results would be of no use, but
-// every thread would still come to the same barriers.
-template <int kWarps>
-__device__ __forceinline__ i32 agreed_label(RowWalk& w, i32 (&labels)[2][32], u32& buffer, u32 rank, u32 blocks) {
-  if constexpr (kWarps == 1) {
-    if (blocks == 1) return w.here();
-  }
-  if (w.at == 32) {
-    buffer ^= 1;  // (slower threads may still read the last 32)
-    w.at = 0;
-    if (rank == 0 && threadIdx.x < 32) {
-      const i32 mine = w.load();
-      for (u32 b = 0; b < blocks; ++b) cluster_put(&labels[buffer][threadIdx.x], b, mine);
-    }
-    if (blocks > 1) {
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();
-    } else {
-      __syncthreads();
-    }
-  }
-  return labels[buffer][w.at];
 }
 
 // One block's share [j0, j1) of a row's whole vectors, in groups of NT * U.
@@ -565,178 +514,166 @@ struct RowShare {
 };
 
 template <class T, bool kPolicy, int NT, int U, int S, int kPerSM>
-__global__ void __launch_bounds__(NT, kPerSM) k_row_loss_ring(RowArgs a, u32 blocks, u32 clusters) {
+__global__ void __launch_bounds__(NT, kPerSM) k_row_loss_ring(RowArgs a, u32 blocks) {
   constexpr int kWarps = NT / 32;
   extern __shared__ uint4 ring[];  // [S][U][NT]
-  __shared__ float2 warp_part[2][kWarps];
-  __shared__ float2 block_part[2][kMaxCluster];
-  __shared__ float row_c[2];
-  __shared__ i32 labels[2][32];
+  __shared__ float2 warp_part[kWarps];
+  __shared__ float2 block_part[kMaxCluster];
+  __shared__ float row_c;
+  __shared__ i32 row_label;
   const u32 t = threadIdx.x, rank = blocks > 1 ? cluster_rank() : 0;
-  const u64 first = blocks > 1 ? blockIdx.x / blocks : blockIdx.x;
-  const T* const z = static_cast<const T*>(a.m.z);
-  if (blocks > 1) {  // every block runs before another one writes to its memory
+  const u64 r = blocks > 1 ? blockIdx.x / blocks : blockIdx.x;
+  // Whether the row has a label decides which barriers its threads meet at, so
+  // one thread reads it for all of them: were the labels written while the
+  // kernel runs, the results would be of no use, but every thread would still
+  // come to the same barriers.
+  i32 y;
+  if (blocks > 1) {
+    cluster_arrive();  // (every block runs before another one writes to its memory)
+    cluster_wait();
+    if (rank == 0 && t < 32) {
+      const i32 mine = __shfl_sync(0xffffffffu, a.label[r], 0);
+      if (t < blocks) cluster_put(&row_label, t, mine);
+      __syncwarp();
+    }
     cluster_arrive();
     cluster_wait();
+    y = row_label;
+  } else if (kWarps > 1) {
+    if (t == 0) row_label = a.label[r];
+    __syncthreads();
+    y = row_label;
+  } else {
+    y = __shfl_sync(0xffffffffu, a.label[r], 0);
   }
-  const bool backward = kPolicy && a.out.grad != nullptr;
-
-  // the copies' place: row, next vectors, groups left, and whether the row
-  // comes once more
-  RowWalk in_rows(a, first, clusters);
-  RowShare<T, NT, U> in_share;
-  const uint4* in_base = nullptr;
+  const bool live = u32(y) < a.m.classes, backward = kPolicy && a.out.grad != nullptr;
+  const RowCut<T> cut(static_cast<const T*>(a.m.z) + r * a.m.stride, a.m.classes);
+  const RowShare<T, NT, U> share(cut, rank, blocks);
+  const u32 n = share.j1 - share.j0, groups = share.groups();
+  const bool ragged = rank == 0 && (cut.head || cut.tail < cut.K);
+  if (!live) {
+    skip_row<kPolicy>(a, r, rank == 0 && t == 0);
+    if constexpr (kPolicy) {
+      if (!backward) return;
+      const RowOut<T> out(a.out, r, cut.shift);
+      const RowCoef none{0.f, 0.f, 0.f, 0.f};
+      if (ragged) cut.template edges<NT>(t, [&](u32 k) { grad_element(out, cut, k, y, none); });
+      for (u32 j = share.j0 + t; j < share.j1; j += NT) out.zero(j);
+    }
+    return;
+  }
+  const bool again = backward && groups > S;  // the ring does not hold the share
+  const uint4* const from = reinterpret_cast<const uint4*>(cut.base) + share.j0 + t;
   const u32 ring_at = u32(__cvta_generic_to_shared(ring + t));
-  u32 in_j = 0, in_left = 0, in_slot = 0;
-  bool again = false;
+  u32 in_group = 0, in_slot = 0, in_left = again ? 2 * groups : groups;
   auto issue = [&]() {
-    if (in_left == 0 && again) {
-      again = false;
-      in_j = in_share.j0 + t;
-      in_left = in_share.groups();
-    }
-    while (in_left == 0 && !in_rows.done()) {
-      if (u32(in_rows.here()) < a.m.classes) {
-        const RowCut<T> cut(z + in_rows.r * a.m.stride, a.m.classes);
-        in_base = reinterpret_cast<const uint4*>(cut.base);
-        in_share = RowShare<T, NT, U>(cut, rank, blocks);
-        in_j = in_share.j0 + t;
-        in_left = in_share.groups();
-        again = backward && in_left > S;
-      }
-      in_rows.next();
-    }
     if (in_left) {
-      const uint4* const from = in_base + in_j;
-      const u32 to = ring_at + in_slot * (U * NT * 16);
-      if (in_left > 1) {
+      const uint4* const src = from + u64(in_group) * (U * NT);
+      const u32 to = ring_at + in_slot * (U * NT * 16), left = n - in_group * (U * NT);
+      if (left >= U * NT) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) copy_async(to + u * (NT * 16), from + u * NT);
+        for (int u = 0; u < U; ++u) copy_async(to + u * (NT * 16), src + u * NT);
       } else {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (in_j + u * NT < in_share.j1) copy_async(to + u * (NT * 16), from + u * NT);
+          if (t + u * NT < left) copy_async(to + u * (NT * 16), src + u * NT);
       }
-      in_j += U * NT;
+      in_group = in_group + 1 == groups ? 0 : in_group + 1;
+      in_slot = in_slot + 1 == S ? 0 : in_slot + 1;
       --in_left;
     }
     copy_commit();  // (empty groups too: the count of groups under way stays S)
-    in_slot = in_slot + 1 == S ? 0 : in_slot + 1;
   };
-#pragma unroll 1
+#pragma unroll
   for (int i = 0; i < S; ++i) issue();
 
-  u32 slot = 0, parity = 0, buffer = 0;
-  for (RowWalk rows(a, first, clusters); !rows.done(); rows.next()) {
-    const u64 r = rows.r;
-    const i32 y = agreed_label<kWarps>(rows, labels, buffer, rank, blocks);
-    const RowCut<T> cut(z + r * a.m.stride, a.m.classes);
-    const RowShare<T, NT, U> share(cut, rank, blocks);
-    const u32 groups = share.groups();
-    const bool live = u32(y) < a.m.classes, stays = backward && groups <= S;
-    const bool ragged = rank == 0 && (cut.head || cut.tail < cut.K);
-    RowCoef q{0.f, 0.f, 0.f, 0.f};
-    float zy = 0.f;
-    if (live) {
-      RowScalars x;
-      zy = to_f32(cut.z[y]);
-      if (t < 32) {
-        x = policy_scalars<kPolicy>(a, r);
-        x.zy = zy;
-      }
-      float m = neg_inf(), s = 0.f;
-      if (ragged) cut.template edges<NT>(t, [&](u32 k) { join_element(to_f32(cut.z[k]), m, s); });
-      u32 at = slot;
+  RowScalars x;
+  const float zy = to_f32(cut.z[y]);
+  if (t < 32) {
+    x = policy_scalars<kPolicy>(a, r);
+    x.zy = zy;
+  }
+  float m = neg_inf(), s = 0.f;
+  if (ragged) cut.template edges<NT>(t, [&](u32 k) { join_element(to_f32(cut.z[k]), m, s); });
+  const bool stays = backward && !again;
+  u32 slot = 0;
 #pragma unroll 1
-      for (u32 i = 0; i < groups; ++i) {
-        copy_wait<S>(stays ? S - 1 - i : S - 1);
-        const uint4* const from = ring + at * (U * NT) + t;
-        const u32 left = share.j1 - share.j0 - i * (U * NT);
-        if (left >= U * NT) {
-          uint4 v[U];
+  for (u32 i = 0; i < groups; ++i) {
+    copy_wait<S>(stays ? S - 1 - i : S - 1);
+    const uint4* const at = ring + slot * (U * NT) + t;
+    const u32 left = n - i * (U * NT);
+    if (left >= U * NT) {
+      uint4 v[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) v[u] = from[u * NT];
-          join_vectors<T, U>(v, m, s);
-        } else {  // the last, short group: only as many vectors as there are
+      for (int u = 0; u < U; ++u) v[u] = at[u * NT];
+      join_vectors<T, U>(v, m, s);
+    } else {  // the last, short group: only as many vectors as there are
 #pragma unroll 1
-          for (u32 k = t; k - t < left; k += NT) {
-            const uint4 v[1] = {k < left ? from[k - t] : Vec<T>::none()};
-            join_vectors<T, 1>(v, m, s);
-          }
-        }
-        at = at + 1 == S ? 0 : at + 1;
-        if (!stays) {
-          issue();
-          slot = at;
-        }
+      for (u32 k = t; k - t < left; k += NT) {
+        const uint4 v[1] = {k < left ? at[k - t] : Vec<T>::none()};
+        join_vectors<T, 1>(v, m, s);
       }
-      // the pairs of the threads, then of the warps (every warp alike), then of the blocks
-      const float wm = lanes_reduce<32>(m, MaxOp());
-      s = lanes_reduce<32>(rebase(s, m, wm), SumOp());
-      m = wm;
-      if constexpr (kWarps > 1) {
-        if ((t & 31) == 0) warp_part[parity][t >> 5] = make_float2(m, s);
-        __syncthreads();
-        const float2 p = warp_part[parity][t & (kWarps - 1)];
-        m = lanes_reduce<kWarps>(p.x, MaxOp());
-        s = lanes_reduce<kWarps>(rebase(p.y, p.x, m), SumOp());
-      }
-      if (blocks > 1) cluster_join(block_part[parity], blocks, m, s);
-      // the loss and its derivative are one warp's work
-      if (t < 32) {
-        q.c = finish_row<kPolicy>(a, r, x, m, s, rank == 0 && t == 0);
-        if (kWarps > 1 && t == 0) row_c[parity] = q.c;
-      }
-      if (kWarps > 1 && backward) {
-        __syncthreads();
-        q.c = row_c[parity];
-      }
-      parity ^= 1;  // (a row's parts are written while slower threads read the last row's)
-      q.base = exp_base(m);
-      q.scale = inverse(s);
+    }
+    slot = slot + 1 == S ? 0 : slot + 1;
+    if (!stays) issue();
+  }
+  // the pairs of the threads, then of the warps (every warp alike), then of the blocks
+  const float wm = lanes_reduce<32>(m, MaxOp());
+  s = lanes_reduce<32>(rebase(s, m, wm), SumOp());
+  m = wm;
+  if constexpr (kWarps > 1) {
+    if ((t & 31) == 0) warp_part[t >> 5] = make_float2(m, s);
+    __syncthreads();
+    const float2 p = warp_part[t & (kWarps - 1)];
+    m = lanes_reduce<kWarps>(p.x, MaxOp());
+    s = lanes_reduce<kWarps>(rebase(p.y, p.x, m), SumOp());
+  }
+  if (blocks > 1) cluster_join(block_part, blocks, m, s);
+  // the loss and its derivative are one warp's work
+  RowCoef q{0.f, exp_base(m), 0.f, inverse(s)};
+  if (t < 32) {
+    q.c = finish_row<kPolicy>(a, r, x, m, s, rank == 0 && t == 0);
+    if (kWarps > 1 && t == 0) row_c = q.c;
+  }
+  if constexpr (kPolicy) {
+    if (!backward) return;
+    if constexpr (kWarps > 1) {
+      __syncthreads();
+      q.c = row_c;
     } else {
-      skip_row<kPolicy>(a, r, rank == 0 && t == 0);
+      __syncwarp();  // (in place: the label's margin has been read)
     }
-    if constexpr (kPolicy) {
-      if (!backward) continue;
-      if constexpr (kWarps == 1) __syncwarp();  // (in place: the label's margin has been read)
-      const RowOut<T> out(a.out, r, cut.shift);
-      if (ragged) cut.template edges<NT>(t, [&](u32 k) { grad_element(out, cut, k, y, q); });
-      if (q.c == 0.f) {
-        for (u32 j = share.j0 + t; j < share.j1; j += NT) out.zero(j);
-        if (live) {
-          for (u32 i = 0; i < groups; ++i) {
-            if (!stays) copy_wait<S>(S - 1);
-            issue();
-            slot = slot + 1 == S ? 0 : slot + 1;
-          }
-        }
-        continue;
-      }
-      u32 j = share.j0 + t;
+    const RowOut<T> out(a.out, r, cut.shift);
+    if (ragged) cut.template edges<NT>(t, [&](u32 k) { grad_element(out, cut, k, y, q); });
+    u32 j = share.j0 + t;
+    if (q.c == 0.f) {
+      copy_wait<1>(0);  // (a block does not end with copies under way)
+      for (; j < share.j1; j += NT) out.zero(j);
+      return;
+    }
+    if (stays) slot = 0;
 #pragma unroll 1
-      for (u32 i = 0; i < groups; ++i) {
-        if (!stays) copy_wait<S>(S - 1);
-        const uint4* const from = ring + slot * (U * NT) + t;
-        if (share.j1 - (j - t) >= U * NT) {
-          uint4 v[U];
+    for (u32 i = 0; i < groups; ++i) {
+      if (again) copy_wait<S>(S - 1);
+      const uint4* const at = ring + slot * (U * NT) + t;
+      if (share.j1 - (j - t) >= U * NT) {
+        uint4 v[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) v[u] = from[u * NT];
-          grad_vectors<T, U, NT>(out, j, share.j1, v, q);
-        } else {
+        for (int u = 0; u < U; ++u) v[u] = at[u * NT];
+        grad_vectors<T, U, NT>(out, j, share.j1, v, q);
+      } else {
 #pragma unroll 1
-          for (u32 k = j; k < share.j1; k += NT) {
-            uint4 v[1] = {from[k - j]};
-            grad_vectors<T, 1, NT>(out, k, share.j1, v, q);
-          }
+        for (u32 k = j; k < share.j1; k += NT) {
+          uint4 v[1] = {at[k - j]};
+          grad_vectors<T, 1, NT>(out, k, share.j1, v, q);
         }
-        j += U * NT;
-        issue();
-        slot = slot + 1 == S ? 0 : slot + 1;
       }
-      const u32 jy = cut.vector_of(u32(y));
-      if (jy >= share.j0 && jy < share.j1 && (jy - share.j0) % NT == t) grad_label(out, cut, y, zy, q);
+      j += U * NT;
+      slot = slot + 1 == S ? 0 : slot + 1;
+      if (again) issue();
     }
+    const u32 jy = cut.vector_of(u32(y));
+    if (jy >= share.j0 && jy < share.j1 && (jy - share.j0) % NT == t) grad_label(out, cut, y, zy, q);
   }
 }
 
@@ -1004,7 +941,6 @@ __global__ void __launch_bounds__(256) k_row_thread(TileArgs t) {
 
 // ---- launches ---------------------------------------------------------------
 constexpr u32 kSMs = 148;
-constexpr int kMaxDevices = 16;
 inline u32 grid_of(u64 blocks) {
   need(blocks < (u64(1) << 31), "too many rows for one launch");
   return u32(blocks);
@@ -1098,8 +1034,10 @@ void launch_ring(const RowArgs& a, u32 blocks, cudaStream_t s) {
   constexpr u32 kShared = u32(NT) * U * S * 16;
   static_assert(kShared * kPerSM <= 220 * 1024, "the rings of an SM's blocks exceed its shared memory");
   auto* const kernel = k_row_loss_ring<T, kPolicy, NT, U, S, kPerSM>;
+  if (kShared > 40 * 1024)  // (with the static arrays above the 48 KB that need no leave)
+    DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kShared)));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
+  cfg.gridDim = dim3(grid_of(a.m.rows * blocks));
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = kShared;
   cfg.stream = s;
@@ -1109,26 +1047,7 @@ void launch_ring(const RowArgs& a, u32 blocks, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = blocks > 1 ? 1 : 0;
-  // one cluster for every place that the device has for one (clusters do not
-  // fill it evenly), asked for once a device and cluster size
-  static std::atomic<int> places[kMaxDevices][kMaxCluster + 1];
-  int dev = 0;
-  DP_CUDA(cudaGetDevice(&dev));
-  int fit = dev < kMaxDevices ? places[dev][blocks].load(std::memory_order_relaxed) : 0;
-  if (fit == 0) {
-    DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kShared)));
-    if (blocks > 1) {
-      DP_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
-    } else {
-      DP_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, NT, kShared));
-      fit *= int(kSMs);
-    }
-    need(fit > 0, "the device has no place for a row's blocks");
-    if (dev < kMaxDevices) places[dev][blocks].store(fit, std::memory_order_relaxed);
-  }
-  const u32 clusters = u32(a.m.rows < u64(fit) ? a.m.rows : u64(fit));
-  cfg.gridDim = dim3(clusters * blocks);
-  DP_CUDA((cudaLaunchKernelEx(&cfg, kernel, a, blocks, clusters)));
+  DP_CUDA((cudaLaunchKernelEx(&cfg, kernel, a, blocks)));
 }
 
 // Blocks of 256 threads a row, at least `blocks`: with few rows, as many as
@@ -1138,27 +1057,33 @@ inline u32 few_rows_cluster(u64 rows, u32 nvec, u32 blocks) {
   return blocks;
 }
 
-// Threads that share a row in the ring kernel.  The fewer, the less of the
-// time goes into joining their sums: about what three and a half vectors a
-// thread take (134M bf16 margins in 16,384 rows: 46 us by 32 threads, 50 by
-// 64, 55 by 128, 57 by 256).  But a row that is to stay for its gradient
-// (`stays`) has to fit in their ring, 16 vectors a thread, and the rows should
-// come out even over the places that the device has for them (4096 rows over
-// 3552 places of 32 threads would leave most idle for half of the time).
-inline u32 ring_threads(u64 rows, u32 nvec, bool stays) {
-  u32 best = 256;
-  double most = 0.0;
-  for (u32 threads = 32; threads <= 256; threads *= 2) {
-    const u64 places = u64(kSMs) * 24 * 32 / threads;
-    if (threads < 256 && ((stays && nvec > threads * 16) || rows * 2 < places)) continue;
-    const double each = double(nvec) / threads;
-    const double share = each / (each + 3.5) * double(rows) / double((rows + places - 1) / places * places);
-    if (share > most) {
-      most = share;
-      best = threads;
-    }
+// The ring kernel's shapes: threads a row and groups of four vectors a thread
+// that their ring holds; as many blocks are resident as the rings leave room
+// for, about 24 warps an SM.
+enum RingShape { kRing32x3, kRing64x2, kRing64x3, kRing64x4, kRing128x4, kRing256x3, kRing256x4 };
+// As few threads as a row keeps busy, for joining their sums costs what about
+// four vectors of each take, but as many as half fill the device.  For the
+// policy loss the smallest ring that holds the row (134M margins of 4096 bf16
+// classes: 92 us by 32 threads x 4 groups and 64 x 3, 103 by 64 x 4; of 3000
+// 94 by 32 x 3, 100 by 32 x 4, 110 by 64 x 3; of 16,384 92 by 128 x 4, 99 by
+// 64 x 4, 104 by 256 x 3); for the log-probability, which only streams, less
+// ring and more rows under way (4096: 43 us by 64 x 2, 48 by 64 x 3, 53 by
+// 64 x 4; 8192 43 by 64 x 3, 49 by 32 x 4; 65,536 45 by 256 x 3, 46 by
+// 128 x 4, 50 by 64 x 3).
+inline RingShape ring_shape(u64 rows, u32 nvec, bool policy) {
+  u32 least = 32;
+  while (least < 256 && rows * least < u64(kSMs) * 384) least *= 2;
+  if (least <= 32 && nvec <= 384) return kRing32x3;
+  if (!policy) {
+    if (least <= 64 && nvec <= 512) return kRing64x2;
+    if (least <= 64 && nvec <= 3072) return kRing64x3;
+    if (least <= 128 && nvec <= 6144) return kRing128x4;
+    return kRing256x3;
   }
-  return best;
+  if (least <= 64 && nvec <= 768) return kRing64x3;
+  if (least <= 64 && nvec <= 1024) return kRing64x4;
+  if (least <= 128 && nvec <= 2048) return kRing128x4;
+  return nvec <= 3072 ? kRing256x3 : kRing256x4;
 }
 
 template <class T, bool kPolicy>
@@ -1184,16 +1109,26 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
     launch_lanes<T, kPolicy, 32>(a, nvec, s);
   } else {
     // (whether a gradient is asked for changes nothing: the loss keeps its bits)
-    switch (ring_threads(a.m.rows, nvec, kPolicy)) {
-      case 32: launch_ring<T, kPolicy, 32, 4, 4, 24>(a, 1, s); break;
-      case 64: launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s); break;
-      case 128: launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s); break;
-      default: {
-        // a row past the ring is cut over a cluster of blocks
-        u32 blocks = 1;
-        while (kPolicy && blocks < kMaxCluster && nvec > blocks * (256u * 4 * 4)) blocks *= 2;
-        launch_ring<T, kPolicy, 256, 4, 4, 3>(a, few_rows_cluster(a.m.rows, nvec, blocks), s);
-      }
+    // A row past two rings, the second read coming from L2, is cut over a
+    // cluster of blocks (134M margins, past one ring and past two: bf16 65,536
+    // classes 119 and 104 us, 131,072 126 and 113; fp32 32,768 202 and 188,
+    // 65,536 213 and 200; past four 65,536 fp32 classes take 276).
+    u32 blocks = 1;
+    while (kPolicy && blocks < kMaxCluster && nvec > blocks * (2u * 256 * 4 * 4)) blocks *= 2;
+    switch (ring_shape(a.m.rows, nvec, kPolicy)) {
+      case kRing32x3: launch_ring<T, kPolicy, 32, 4, 3, 28>(a, 1, s); break;
+      case kRing64x2:
+        if constexpr (!kPolicy) launch_ring<T, kPolicy, 64, 4, 2, 24>(a, 1, s);
+        break;
+      case kRing64x3: launch_ring<T, kPolicy, 64, 4, 3, 16>(a, 1, s); break;
+      case kRing64x4:
+        if constexpr (kPolicy) launch_ring<T, kPolicy, 64, 4, 4, 12>(a, 1, s);
+        break;
+      case kRing128x4: launch_ring<T, kPolicy, 128, 4, 4, 6>(a, 1, s); break;
+      case kRing256x3: launch_ring<T, kPolicy, 256, 4, 3, 4>(a, few_rows_cluster(a.m.rows, nvec, blocks), s); break;
+      case kRing256x4:
+        if constexpr (kPolicy) launch_ring<T, kPolicy, 256, 4, 4, 3>(a, few_rows_cluster(a.m.rows, nvec, blocks), s);
+        break;
     }
   }
   after_launch("row loss");
