@@ -1013,16 +1013,16 @@ bool use_tile(const Margins& m) {
                              !(m.classes * sizeof(T) % 16 == 0 && on_boundaries(m.z, m.rows, m.stride, sizeof(T), 16)));
 }
 
-// (fewer vectors a lane are the next smaller G's)
+// (between 2 and 32 lanes, up to four vectors a lane are the next smaller G's)
 template <class T, bool kPolicy, int G>
 void launch_lanes(const RowArgs& a, u32 nvec, cudaStream_t s) {
   const u32 grid = grid_of((a.m.rows + 256 / G - 1) / (256 / G)), per_lane = (nvec + G - 1) / G;
-  if constexpr (G == 2) {
+  if constexpr (G == 2 || G == 32) {
     if (per_lane <= 2) k_row_loss<T, kPolicy, G, 2><<<grid, 256, 0, s>>>(a);
     else if (per_lane <= 3) k_row_loss<T, kPolicy, G, 3><<<grid, 256, 0, s>>>(a);
     else if (per_lane <= 4) k_row_loss<T, kPolicy, G, 4><<<grid, 256, 0, s>>>(a);
   }
-  if (G > 2 || per_lane > 4) {
+  if ((G != 2 && G != 32) || per_lane > 4) {
     if (per_lane <= 5) k_row_loss<T, kPolicy, G, 5><<<grid, 256, 0, s>>>(a);
     else if (per_lane <= 6) k_row_loss<T, kPolicy, G, 6><<<grid, 256, 0, s>>>(a);
     else k_row_loss<T, kPolicy, G, 8><<<grid, 256, 0, s>>>(a);
@@ -1093,6 +1093,9 @@ void launch_rows_of(const RowArgs& a, cudaStream_t s) {
   const u32 nvec = row_vectors<T>(a.m);
   if (use_tile<T>(a.m)) {
     launch_tile<T, kPolicy ? kTilePolicy : kTileLogProb>(TileArgs{a, nullptr, nullptr}, s);
+  } else if (nvec <= 32 * V && a.m.rows <= 16 * kSMs) {
+    // few rows: a warp each (64 rows of 1000 fp16 classes: 3.1 us, by 16 lanes 4.6)
+    launch_lanes<T, kPolicy, 32>(a, nvec, s);
   } else if (nvec <= 2 * V) {
     // As few lanes as hold the row with up to eight vectors each, for a row's
     // scalars are every lane's work (67M bf16 margins, with up to eight and up
