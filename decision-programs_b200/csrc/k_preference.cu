@@ -33,7 +33,8 @@ __device__ __forceinline__ PairResult pair_result(const PairLoss& a, float diffe
 }
 
 // ---- consecutive items ------------------------------------------------------
-// Every row an item: a thread takes pairs of rows side by side.
+// Every row an item: a thread takes pairs of rows side by side.  Bound by memory:
+// 2M rows in 1M pairs, gradient and curvature, 5.3 us (32 MB, part of it from L2).
 template <bool kWide>
 __global__ void __launch_bounds__(256) k_preference_rows(PairLoss a, u64 rows, u64 pairs) {
   const u64 step = u64(gridDim.x) * blockDim.x, first = u64(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -234,8 +235,10 @@ __global__ void __launch_bounds__(kBlockThreads) k_preference_block(PairLoss a, 
 // that the plan holds sorted by row, a warp taking kPairChunk entries whatever
 // rows they belong to, so that one row in very many pairs costs no more than
 // many rows in few; then the rows that reach over several chunks.  Bound by
-// the random 32-byte sectors of the gathers (two a pair of 4-byte scores, two
-// of 8-byte terms), which L2 serves.
+// the gathers, two of 4-byte scores and two of 8-byte terms a pair, a random
+// sector a lane, of which L1 takes 0.7 to 0.8 a clock and SM: 8M pairs over 1M
+// rows 178 us (82 + 90 + 4).  One thread a row, evaluating each pair from both
+// of its rows, took 258.
 
 __global__ void __launch_bounds__(256) k_gap(const float* score, const float* ref, u64 rows, float* out) {
   for (u64 r = u64(blockIdx.x) * blockDim.x + threadIdx.x; r < rows; r += u64(gridDim.x) * blockDim.x)
