@@ -742,29 +742,38 @@ struct TileArgs {
 enum TileMode { kTileLogProb, kTilePolicy, kTileGrad };
 constexpr u32 kTileClasses = 64;  // the most that its registers hold
 
-// Copies `rows` rows of K elements between memory (`stride` apart) and a tile
-// without gaps; whole vectors when the rows have no gaps either.
-template <class U, bool kIn>
+// Copies `rows` rows of K (at most KT) elements between memory (`stride`
+// apart) and a tile of NT rows without gaps; whole vectors when the rows have
+// no gaps either.
+template <class U, bool kIn, int KT, int NT>
 __device__ __forceinline__ void copy_rows(U* tile, U* mem, u32 rows, u32 K, u64 stride) {
-  const u32 n = rows * K;
+  const u32 n = rows * K, t = threadIdx.x;
   if (stride == K && (reinterpret_cast<std::uintptr_t>(mem) & 15) == 0) {
     constexpr u32 N = 16 / sizeof(U);
-    uint4 *const a = reinterpret_cast<uint4*>(tile), *const b = reinterpret_cast<uint4*>(mem);
-#pragma unroll 4
-    for (u32 j = threadIdx.x; j < n / N; j += blockDim.x) {
-      if (kIn) a[j] = b[j];
-      else b[j] = a[j];
+    constexpr int kMost = (KT * int(sizeof(U)) + 15) / 16;
+    uint4 *const a = reinterpret_cast<uint4*>(tile) + t, *const b = reinterpret_cast<uint4*>(mem) + t;
+    const u32 nv = n / N;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      if (t + i * NT < nv) {
+        if (kIn) copy_async(u32(__cvta_generic_to_shared(a + i * NT)), b + i * NT);
+        else b[i * NT] = a[i * NT];
+      }
     }
-    const u32 e = n / N * N + threadIdx.x;  // (fewer elements than threads are left)
+    const u32 e = nv * N + t;  // (fewer elements than threads are left)
     if (e < n) {
       if (kIn) tile[e] = mem[e];
       else mem[e] = tile[e];
     }
+    if (kIn) {
+      copy_commit();
+      copy_wait<1>(0);
+    }
   } else {
-    const u32 step_row = blockDim.x / K, step_col = blockDim.x % K;
-    u32 row = threadIdx.x / K, col = threadIdx.x % K;
+    const u32 step_row = NT / K, step_col = NT % K;
+    u32 row = t / K, col = t % K;
 #pragma unroll 4
-    for (u32 e = threadIdx.x; e < n; e += blockDim.x) {
+    for (u32 e = t; e < n; e += NT) {
       if (kIn) tile[e] = mem[row * stride + col];
       else mem[row * stride + col] = tile[e];
       row += step_row;
@@ -780,7 +789,6 @@ __device__ __forceinline__ void copy_rows(U* tile, U* mem, u32 rows, u32 K, u64 
 template <TileMode kMode, int KT>
 __device__ __forceinline__ void tile_row(const TileArgs& t, u64 r, u32 K, bool live, RowScalars& x, float2 norm, float& c,
                                          float (&z)[KT]) {
-  constexpr int kStep = KT < 4 ? KT : 4;
   if (!live) {
     if constexpr (kMode != kTileGrad) skip_row<kMode == kTilePolicy>(t.row, r, true);
     c = 0.f;
@@ -796,18 +804,14 @@ __device__ __forceinline__ void tile_row(const TileArgs& t, u64 r, u32 K, bool l
   const Two base(-exp_base(m));
   Two sum(0.f);
 #pragma unroll
-  for (int k4 = 0; k4 < KT; k4 += kStep) {
-    if (KT <= 8 || u32(k4) < K) {
+  for (int k4 = 0; k4 < KT; k4 += 4) {
+    if (KT <= 16 || u32(k4) < K) {
 #pragma unroll
-      for (int k = k4; k < k4 + kStep; k += 2) {
-        if constexpr (KT == 1) {
-          z[0] = ex2(fmaf(z[0] - exp_base(m), kLog2e, low));
-          sum = sum + Two(z[0], 0.f);
-        } else {
-          const Two e = ex2_both(fma(Two(z[k], z[k + 1]) + base, Two(kLog2e), Two(low)));
-          sum = sum + e;
-          e.get(z[k], z[k + 1]);
-        }
+      for (int k = k4; k < (k4 + 4 < KT ? k4 + 4 : KT); k += 2) {
+        const Two e = ex2_both(fma(Two(z[k], k + 1 < KT ? z[k + 1 < KT ? k + 1 : k] : neg_inf()) + base, Two(kLog2e), Two(low)));
+        sum = sum + e;
+        float past;
+        e.get(z[k], k + 1 < KT ? z[k + 1 < KT ? k + 1 : k] : past);
       }
     }
   }
@@ -827,17 +831,27 @@ __device__ __forceinline__ float tile_hess(float up, float least, float p) {
   return h < least ? least : h;  // (a NaN stays one)
 }
 
-// NT rows a block; KT: the most classes.  10 classes, 13.4M fp32 rows: forward
-// and backward 311 us, 4.5 TB/s, bound by instructions (as many as the next
-// larger KT's registers ask for).  kTurn: row lengths that share a
-// factor of 8 or more with the 32 banks, where the threads of a warp would
-// read and write in few of them: each begins its row at a place of its own
-// and goes round.
-template <class T, TileMode kMode, int KT, int NT, bool kTurn>
-__global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread) {
+// Threads of a warp that read the same place of rows `words` words long meet
+// in a bank when they are this far apart.
+__host__ __device__ constexpr u32 bank_spread(u32 words) {
+  u32 spread = 32;
+  while (spread > 1 && words % (64 / spread) == 0) spread /= 2;
+  return spread;
+}
+template <class T>
+__host__ __device__ constexpr u32 row_words(u32 K) {
+  return K * sizeof(T) % 4 ? 1 : u32(K * sizeof(T) / 4);
+}
+// Rows so long that four threads or fewer apart meet: each thread begins its
+// row at a place of its own and goes round.
+constexpr u32 kTurnSpread = 4;
+
+// NT rows a block; KT: the row length (kExact) or the most that it may be.
+template <class T, TileMode kMode, int KT, int NT, bool kExact, bool kTurn>
+__global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread_given) {
   extern __shared__ uint4 tile16[];
   const RowArgs& a = t.row;
-  const u32 K = a.m.classes;
+  const u32 K = kExact ? u32(KT) : a.m.classes, spread = kExact ? bank_spread(row_words<T>(KT)) : spread_given;
   T* const tile = reinterpret_cast<T*>(tile16);
   float* const htile = reinterpret_cast<float*>(tile16 + (NT * K * u32(sizeof(T)) + 15) / 16);
   const u64 r0 = u64(blockIdx.x) * NT, r = r0 + threadIdx.x;
@@ -855,7 +869,7 @@ __global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread) {
       if (!(norm.x == neg_inf() && norm.y == 0.f)) c = t.weight[r];
     }
   }
-  copy_rows<T, true>(tile, const_cast<T*>(static_cast<const T*>(a.m.z)) + r0 * a.m.stride, rows, K, a.m.stride);
+  copy_rows<T, true, KT, NT>(tile, const_cast<T*>(static_cast<const T*>(a.m.z)) + r0 * a.m.stride, rows, K, a.m.stride);
   __syncthreads();
   const bool backward = kMode == kTileGrad || (kMode == kTilePolicy && a.out.grad != nullptr);
   if (in) {
@@ -888,8 +902,8 @@ __global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread) {
   }
   if (!backward) return;
   __syncthreads();
-  copy_rows<T, false>(tile, static_cast<T*>(a.out.grad) + r0 * a.out.grad_stride, rows, K, a.out.grad_stride);
-  if (a.out.hess) copy_rows<float, false>(htile, a.out.hess + r0 * a.out.hess_stride, rows, K, a.out.hess_stride);
+  copy_rows<T, false, KT, NT>(tile, static_cast<T*>(a.out.grad) + r0 * a.out.grad_stride, rows, K, a.out.grad_stride);
+  if (a.out.hess) copy_rows<float, false, KT, NT>(htile, a.out.hess + r0 * a.out.hess_stride, rows, K, a.out.hess_stride);
 }
 
 // A row of B bytes between registers and memory on its boundaries.
@@ -963,18 +977,24 @@ u32 row_vectors(const Margins& m) {
   return m.classes / u32(16 / sizeof(T));
 }
 
-template <class T, TileMode kMode, int KT, int NT>
+template <class T, TileMode kMode, int KT, int NT, bool kExact>
 void launch_tile_of(const TileArgs& t, cudaStream_t s) {
   const u64 K = t.row.m.classes, size = (NT * K * sizeof(T) + 15) / 16 * 16 + (t.row.out.hess ? NT * K * 4 : 0);
-  // lanes `spread` apart would meet in a bank: 32 by the row length's common factor with the banks
-  const u32 words = u32(K * sizeof(T) % 4 ? 1 : K * sizeof(T) / 4);
-  u32 spread = 32;
-  while (spread > 1 && words % (64 / spread) == 0) spread /= 2;
-  auto* kernel = k_row_tile<T, kMode, KT, NT, false>;
-  if constexpr (KT % 8 == 0 && KT * sizeof(T) >= 32)
-    if (spread <= 4) kernel = k_row_tile<T, kMode, KT, NT, true>;
+  const u32 spread = bank_spread(row_words<T>(u32(K)));
+  constexpr bool kMayTurn = kExact ? bank_spread(row_words<T>(KT)) <= kTurnSpread : true;
+  auto* kernel = k_row_tile<T, kMode, KT, NT, kExact, kExact && kMayTurn>;
+  if constexpr (!kExact)
+    if (spread <= kTurnSpread) kernel = k_row_tile<T, kMode, KT, NT, kExact, true>;
   if (size > 48 * 1024) DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(size)));
   kernel<<<grid_of((t.row.m.rows + NT - 1) / NT), NT, size, s>>>(t, spread);
+}
+// Up to 16 classes by their number, so that nothing is spent on classes that
+// are not there (13.4M rows of 10 fp32 classes, forward and backward: @@ us, with
+// one variant for 9 to 12 classes 311).
+template <class T, TileMode kMode, int KT>
+void launch_tile_exact(const TileArgs& t, cudaStream_t s) {
+  if (int(t.row.m.classes) == KT) launch_tile_of<T, kMode, KT, 256, true>(t, s);
+  else if constexpr (KT < 16) launch_tile_exact<T, kMode, KT + 1>(t, s);
 }
 // Whether every row of an array lies on the boundaries of its B bytes.
 inline bool on_boundaries(const void* p, u64 rows, u64 stride, u64 size, u64 B) {
@@ -996,22 +1016,16 @@ void launch_tile(const TileArgs& t, cudaStream_t s) {
     if (K == 4) k_row_thread<T, kMode, 4><<<grid, 256, 0, s>>>(t);
     if (K == 8) k_row_thread<T, kMode, 8><<<grid, 256, 0, s>>>(t);
     if (K == 16) k_row_thread<T, kMode, 16><<<grid, 256, 0, s>>>(t);
-  } else if (K <= 4) {
-    launch_tile_of<T, kMode, 4, 256>(t, s);
-  } else if (K <= 8) {
-    launch_tile_of<T, kMode, 8, 256>(t, s);
-  } else if (K <= 12) {
-    launch_tile_of<T, kMode, 12, 256>(t, s);
   } else if (K <= 16) {
-    launch_tile_of<T, kMode, 16, 256>(t, s);
+    launch_tile_exact<T, kMode, 1>(t, s);
   } else if (K <= 24) {
-    launch_tile_of<T, kMode, 24, 128>(t, s);
+    launch_tile_of<T, kMode, 24, 128, false>(t, s);
   } else if (K <= 32) {
-    launch_tile_of<T, kMode, 32, 128>(t, s);
+    launch_tile_of<T, kMode, 32, 128, false>(t, s);
   } else if (K <= 48) {
-    launch_tile_of<T, kMode, 48, 128>(t, s);
+    launch_tile_of<T, kMode, 48, 128, false>(t, s);
   } else {
-    launch_tile_of<T, kMode, 64, 128>(t, s);
+    launch_tile_of<T, kMode, 64, 128, false>(t, s);
   }
 }
 
