@@ -846,7 +846,9 @@ __host__ __device__ constexpr u32 row_words(u32 K) {
 // row at a place of its own and goes round.
 constexpr u32 kTurnSpread = 4;
 
-// NT rows a block; KT: the row length (kExact) or the most that it may be.
+// NT rows a block; KT: the row length (kExact) or the most that it may be.  fp32
+// rows are bound by DRAM (6.7M x 10, forward and backward: 107 us, 6.5 TB/s),
+// 16-bit ones by instructions (the same in bf16: 92 us, 3.8 TB/s).
 template <class T, TileMode kMode, int KT, int NT, bool kExact, bool kTurn>
 __global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread_given) {
   extern __shared__ uint4 tile16[];
@@ -989,8 +991,8 @@ void launch_tile_of(const TileArgs& t, cudaStream_t s) {
   kernel<<<grid_of((t.row.m.rows + NT - 1) / NT), NT, size, s>>>(t, spread);
 }
 // Up to 16 classes by their number, so that nothing is spent on classes that
-// are not there (13.4M rows of 10 fp32 classes, forward and backward: @@ us, with
-// one variant for 9 to 12 classes 311).
+// are not there (6.7M rows of 10 fp32 classes, forward and backward: 107 us; with
+// one variant for 9 to 12 classes, and copies in loops, 161).
 template <class T, TileMode kMode, int KT>
 void launch_tile_exact(const TileArgs& t, cudaStream_t s) {
   if (int(t.row.m.classes) == KT) launch_tile_of<T, kMode, KT, 256, true>(t, s);
@@ -1018,25 +1020,34 @@ void launch_tile(const TileArgs& t, cudaStream_t s) {
     if (K == 16) k_row_thread<T, kMode, 16><<<grid, 256, 0, s>>>(t);
   } else if (K <= 16) {
     launch_tile_exact<T, kMode, 1>(t, s);
+  } else if (K <= 20) {
+    launch_tile_of<T, kMode, 20, 128, false>(t, s);
   } else if (K <= 24) {
     launch_tile_of<T, kMode, 24, 128, false>(t, s);
+  } else if (K <= 28) {
+    launch_tile_of<T, kMode, 28, 128, false>(t, s);
   } else if (K <= 32) {
     launch_tile_of<T, kMode, 32, 128, false>(t, s);
+  } else if (K <= 40) {
+    launch_tile_of<T, kMode, 40, 128, false>(t, s);
   } else if (K <= 48) {
     launch_tile_of<T, kMode, 48, 128, false>(t, s);
+  } else if (K <= 56) {
+    launch_tile_of<T, kMode, 56, 128, false>(t, s);
   } else {
     launch_tile_of<T, kMode, 64, 128, false>(t, s);
   }
 }
 
-// One thread a row up to 16 classes; up to 64 also where rows lie off the
-// 16-byte boundaries, which lanes would take element by element at both ends
-// (67M margins, lanes and tile: 64 bf16 classes 61 and 131 us, 33 145 and 104;
-// fp32 104 and 145, 150 and 127).
+// One thread a row up to 36 fp32 or 24 16-bit classes (67M margins, one thread
+// and lanes: 36 fp32 classes 101 and 117 us forward and backward, 40 104 and
+// 96; 24 bf16 classes 86 and 105, 32 103 and 82); up to 64 where rows lie off
+// the 16-byte boundaries, which lanes would take element by element at both
+// ends (33 bf16 classes 79 and 145 us, fp32 92 and 150).
 template <class T>
 bool use_tile(const Margins& m) {
-  return m.classes <= 16 || (m.classes <= kTileClasses &&
-                             !(m.classes * sizeof(T) % 16 == 0 && on_boundaries(m.z, m.rows, m.stride, sizeof(T), 16)));
+  const bool even = m.classes * sizeof(T) % 16 == 0 && on_boundaries(m.z, m.rows, m.stride, sizeof(T), 16);
+  return m.classes <= (!even ? kTileClasses : sizeof(T) == 4 ? 36 : 24);
 }
 
 // (between 2 and 32 lanes, up to four vectors a lane are the next smaller G's)
