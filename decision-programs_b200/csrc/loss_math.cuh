@@ -98,9 +98,11 @@ __device__ __forceinline__ float policy_row(const PolicyRows& p, const RowScalar
 
 // Gradient and curvature of c * log p(label) by one margin of probability p.
 __device__ __forceinline__ float margin_grad(float c, float p, bool chosen) { return c * ((chosen ? 1.f : 0.f) - p); }
-// The softmax objective's diagonal form, with its factor 2 and its floor.
-__device__ __forceinline__ float margin_hess(float c, float p) {
-  return fabsf(c) * fmaxf(2.f * p * (1.f - p), 1e-16f);
+// The softmax objective's diagonal form, |c| max(2 p (1 - p), 1e-16), for
+// size = |c|; the comparison lets a NaN through.
+__device__ __forceinline__ float margin_hess(float size, float p) {
+  const float least = size * 1e-16f, h = (1.f - p) * p * (size + size);
+  return h < least ? least : h;
 }
 
 // Preference loss of a pair at x = beta * (gap of scores): the loss, its

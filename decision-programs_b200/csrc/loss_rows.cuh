@@ -227,13 +227,12 @@ __device__ __forceinline__ void grad_vector(const RowOut<T>& out, u32 j, const u
   for (int i = 0; i < P; ++i) e[i] = f[i] * Two(-q.c * q.scale);
   out.store(j, Vec<T>::pack(e));
   if (out.h) {
-    const float ac = fabsf(q.c), least = ac * 1e-16f;
+    const float size = fabsf(q.c), least = size * 1e-16f;  // (margin_hess on pairs)
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const Two p = f[i] * Two(q.scale);
       float a, b;
-      (fma(p, Two(-1.f), Two(1.f)) * p * Two(2.f * ac)).get(a, b);
-      // (the comparison lets a NaN through)
+      (fma(p, Two(-1.f), Two(1.f)) * p * Two(2.f * size)).get(a, b);
       e[i] = Two(a < least ? least : a, b < least ? least : b);
     }
     out.store_hess(j, e);
@@ -282,7 +281,7 @@ __device__ __forceinline__ void grad_element(const RowOut<T>& out, const RowCut<
   if (q.c != 0.f) {
     const float p = q.p(to_f32(cut.z[k]));
     gv = margin_grad(q.c, p, k == u32(y));
-    hv = margin_hess(q.c, p);
+    hv = margin_hess(fabsf(q.c), p);
   }
   out.put(cut.shift, k, gv, hv);
 }
@@ -825,12 +824,6 @@ __device__ __forceinline__ void tile_row(const TileArgs& t, u64 r, u32 K, bool l
     for (int k = 0; k < KT; ++k) z[k] *= scale;
   }
 }
-// The row's curvature by one probability.
-__device__ __forceinline__ float tile_hess(float up, float least, float p) {
-  const float h = (1.f - p) * p * (up + up);
-  return h < least ? least : h;  // (a NaN stays one)
-}
-
 // Threads of a warp that read the same place of rows `words` words long meet
 // in a bank when they are this far apart.
 __host__ __device__ constexpr u32 bank_spread(u32 words) {
@@ -889,13 +882,13 @@ __global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread_given) {
     if (backward) {
       float* const mine_h = htile + threadIdx.x * K;
       const bool none = c == 0.f, hess = a.out.hess != nullptr;
-      const float up = fabsf(c), least = up * 1e-16f, down = -c;
+      const float size = fabsf(c), down = -c;
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         if (u32(k) < K) {
           const u32 at = place(k);
           mine[at] = from_f32<T>(none ? 0.f : down * z[k]);
-          if (hess) mine_h[at] = none ? 0.f : tile_hess(up, least, z[k]);
+          if (hess) mine_h[at] = none ? 0.f : margin_hess(size, z[k]);
           if (at == u32(y)) c = none ? 0.f : c - c * z[k];
         }
       }
@@ -958,10 +951,10 @@ __global__ void __launch_bounds__(256) k_row_thread(TileArgs t) {
   memcpy(&raw, v, sizeof v);
   raw.store(static_cast<T*>(a.out.grad) + r * a.out.grad_stride);
   if (a.out.hess) {
-    const float up = fabsf(c), least = up * 1e-16f;
+    const float size = fabsf(c);
     RowBytes<K * 4> h;
 #pragma unroll
-    for (int k = 0; k < K; ++k) z[k] = none ? 0.f : tile_hess(up, least, z[k]);
+    for (int k = 0; k < K; ++k) z[k] = none ? 0.f : margin_hess(size, z[k]);
     memcpy(&h, z, sizeof z);
     h.store(a.out.hess + r * a.out.hess_stride);
   }
@@ -987,7 +980,9 @@ void launch_tile_of(const TileArgs& t, cudaStream_t s) {
   auto* kernel = k_row_tile<T, kMode, KT, NT, kExact, kExact && kMayTurn>;
   if constexpr (!kExact)
     if (spread <= kTurnSpread) kernel = k_row_tile<T, kMode, KT, NT, kExact, true>;
-  if (size > 48 * 1024) DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(size)));
+  constexpr int kMost = NT * KT * (int(sizeof(T)) + 4) + 16;  // (one value for every call: other threads launch too)
+  if constexpr (kMost > 48 * 1024)
+    if (size > 48 * 1024) DP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
   kernel<<<grid_of((t.row.m.rows + NT - 1) / NT), NT, size, s>>>(t, spread);
 }
 // Up to 16 classes by their number, so that nothing is spent on classes that
