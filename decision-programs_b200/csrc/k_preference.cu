@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kBlockThreads) k_preference_block(PairLoss a, 
 // many rows in few; then the rows that reach over several chunks.  Bound by
 // the gathers, two of 4-byte scores and two of 8-byte terms a pair, a random
 // sector a lane, of which L1 takes 0.7 to 0.8 a clock and SM: 8M pairs over 1M
-// rows 178 us (82 + 90 + 4).  One thread a row, evaluating each pair from both
+// rows 170 us (82 + 83 + 5).  One thread a row, evaluating each pair from both
 // of its rows, took 258.
 
 __global__ void __launch_bounds__(256) k_gap(const float* score, const float* ref, u64 rows, float* out) {
