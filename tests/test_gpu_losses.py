@@ -117,7 +117,8 @@ def check_rows(dp, z, z64, y, rng, dtype, hess=True, in_place=False, weight=None
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("classes", [1, 2, 3, 4, 7, 8, 9, 10, 16, 17, 31, 32, 33, 47, 64, 65, 96, 100, 127, 128, 129, 255,
+@pytest.mark.parametrize("classes", [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 20, 21, 24, 25, 28, 29, 31,
+                                     32, 33, 36, 37, 40, 41, 47, 48, 49, 56, 57, 63, 64, 65, 96, 100, 127, 128, 129, 255,
                                      256, 257, 511, 513, 1000, 1024, 1025])
 def test_small_class_counts(dp, dtype, classes):
     rows = 203 if classes < 200 else 37
@@ -144,6 +145,16 @@ def test_row_counts(dp, dtype, rows, classes):
     weight = rng.random(rows).astype(np.float32)
     weight[rng.random(rows) < 0.2] = 0.0
     check_rows(dp, z, z64, labels(rng, rows, classes), rng, dtype, weight=weight)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [24, 40, 64, 65, 72, 96, 127, 128, 160, 200, 256, 257, 320, 500, 512, 640, 1000, 1024])
+def test_many_rows(dp, dtype, classes):
+    """Rows past the count where each gets a warp: 2 to 32 lanes a row."""
+    rows = 2501
+    for pad, shift in ((0, 0), (5, 2)) if classes < 300 else ((0, 0),):
+        z, z64, rng = margins(rows, classes, dtype, 3 * classes + pad, pad, shift)
+        check_rows(dp, z, z64, labels(rng, rows, classes), rng, dtype, hess=classes % 3 != 0, in_place=pad > 0)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
