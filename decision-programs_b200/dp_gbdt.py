@@ -535,13 +535,13 @@ def _grad_out(margin, grad, hess):
     """The gradient and curvature tensors of a call, and their arguments."""
     import torch
     if grad is None or grad is True:
-        grad = torch.empty(margin.shape, dtype=margin.dtype, device=margin.device)
+        grad = torch.empty_like(margin)  # (margins whose rows lie apart: without the gaps)
     else:
         _need(grad.shape == margin.shape and grad.dtype == margin.dtype and grad.device == margin.device,
               "grad must have the margins' shape, type and device")
     if not hess:
         return grad, None, (*_rows_of(grad, "grad"), None, 0)
-    hess = torch.empty(margin.shape, dtype=torch.float32, device=margin.device)
+    hess = torch.empty_like(margin, dtype=torch.float32)
     return grad, hess, (*_rows_of(grad, "grad"), *_rows_of(hess, "hess"))
 
 
