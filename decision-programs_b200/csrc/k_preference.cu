@@ -229,6 +229,96 @@ __global__ void __launch_bounds__(kBlockThreads) k_preference_block(PairLoss a, 
   fill_outside(a, rows, begin, pairs);
 }
 
+// Few pairs of very many rows: every block of the device takes pieces of
+// kPieceRows rows, whatever pairs they belong to, in three launches, since a
+// pair's one cluster of blocks uses eight SMs alone (reference scores given, by
+// pieces against by clusters: 4M rows in one pair 16.5 us against 84, one pair
+// of 262,144 rows 8.8 / 9.9, of 131,072 8.3 / 7.6; eight pairs of 262,144 rows
+// each 14.8 / 14.6, with the curvature 16.2 / 20.2; sixteen of them 33.9 /
+// 27.5).  The pieces' sums wait in the gradient's place, which has two rows or
+// more for each piece of a pair of kPiecedRows rows; shorter pairs are summed
+// by the second launch.  It leaves a pair's gradient (and curvature) in its
+// first row, where the third finds it for the others.
+constexpr u32 kPieceRows = 8192, kPiecedRows = 4 * kPieceRows, kFewPairs = 8;
+constexpr u64 kVeryLongRows = u64(1) << 18;  // a pair, on average
+struct PairSpan {
+  u64 b0, b1, b2;
+  __device__ __forceinline__ PairSpan(const u64* offset, u64 p) : b0(offset[2 * p]), b1(offset[2 * p + 1]), b2(offset[2 * p + 2]) {}
+  __device__ __forceinline__ bool pieced() const { return b2 > b0 && b2 - b0 >= kPiecedRows && b1 >= b0 && b1 <= b2; }
+  // Places of a piece's two sums in the gradient.
+  __device__ __forceinline__ u64 place(u64 piece) const { return b0 + 2 * (piece - b0 / kPieceRows); }
+};
+// The offsets, read once for the whole block.
+__device__ __forceinline__ void read_offsets(u64* offset, const i64* begin, u64 pairs, u64 rows) {
+  for (u64 i = threadIdx.x; i <= 2 * pairs; i += blockDim.x) offset[i] = clamp_row(begin[i], rows);
+  __syncthreads();
+}
+// Sums of v over the block's threads, the same in each of them.
+template <int kWarps>
+__device__ __forceinline__ float2 block_sums(float2 v, float2* part) {
+  v.x = lanes_sum<32>(v.x);
+  v.y = lanes_sum<32>(v.y);
+  __syncthreads();  // (the last call's parts have been read)
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[threadIdx.x & (kWarps - 1)];
+  return make_float2(lanes_sum<kWarps>(v.x), lanes_sum<kWarps>(v.y));
+}
+__global__ void __launch_bounds__(512) k_preference_pieces(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
+  __shared__ float2 part[16];
+  __shared__ u64 offset[2 * kFewPairs + 1];
+  read_offsets(offset, begin, pairs, rows);
+  const u64 piece = blockIdx.x, r0 = piece * kPieceRows, r1 = min(rows, r0 + kPieceRows);
+  for (u64 p = 0; p < pairs; ++p) {
+    const PairSpan x(offset, p);
+    if (!x.pieced() || x.b2 <= r0 || x.b0 >= r1) continue;
+    const u64 lo = max(x.b0, r0), hi = min(x.b2, r1), mid = min(max(x.b1, lo), hi);
+    const float2 s = block_sums<16>(make_float2(span_sum<8>(a, lo, mid, threadIdx.x, 512),
+                                                span_sum<8>(a, mid, hi, threadIdx.x, 512)), part);
+    if (threadIdx.x < 2) a.grad[x.place(piece) + threadIdx.x] = threadIdx.x ? s.y : s.x;
+  }
+}
+__global__ void __launch_bounds__(512) k_preference_settle(PairLoss a, u64 rows, const i64* begin) {
+  __shared__ float2 part[16];
+  __shared__ u64 offset[2 * kFewPairs + 1];
+  read_offsets(offset, begin, gridDim.x, rows);
+  const u64 p = blockIdx.x;
+  const PairSpan x(offset, p);
+  float2 s = make_float2(0.f, 0.f);
+  if (x.pieced()) {
+    for (u64 k = x.b0 / kPieceRows + threadIdx.x; k * kPieceRows < x.b2; k += 512) {
+      const u64 at = x.place(k);
+      s.x += a.grad[at];
+      s.y += a.grad[at + 1];
+    }
+  } else {
+    s.x = span_sum<8>(a, x.b0, x.b1, threadIdx.x, 512);
+    s.y = span_sum<8>(a, x.b1, x.b2, threadIdx.x, 512);
+  }
+  s = block_sums<16>(s, part);  // (and every piece's sums have been read)
+  if (threadIdx.x) return;
+  const PairResult o = pair_result(a, s.x - s.y, a.weight ? a.weight[p] : 1.f);
+  a.loss[p] = o.loss;
+  if (x.b2 <= x.b0) return;
+  a.grad[x.b0] = x.b1 > x.b0 ? o.q : -o.q;
+  if (a.hess) a.hess[x.b0] = item_hess(o.h);
+}
+__global__ void __launch_bounds__(512) k_preference_spread(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
+  __shared__ u64 offset[2 * kFewPairs + 1];
+  read_offsets(offset, begin, pairs, rows);
+  const u64 r0 = u64(blockIdx.x) * kPieceRows, r1 = min(rows, r0 + kPieceRows);
+  for (u64 p = 0; p < pairs; ++p) {
+    const PairSpan x(offset, p);
+    const u64 lo = max(x.b0 + 1, r0), hi = min(x.b2, r1);
+    if (lo >= hi) continue;
+    const float first = a.grad[x.b0], q = x.b1 > x.b0 ? first : -first, h = a.hess ? a.hess[x.b0] : 0.f;
+    const u64 mid = min(max(x.b1, lo), hi);
+    span_fill(a, lo, mid, threadIdx.x, 512, q, h);
+    span_fill(a, mid, hi, threadIdx.x, 512, -q, h);
+  }
+  fill_outside(a, rows, begin, pairs);
+}
+
 // ---- any pairs --------------------------------------------------------------
 // Three launches: every pair's terms once, in the pairs' order (two gathers of
 // scores a pair); then the terms summed by row over the list of (row, pair)
@@ -536,10 +626,18 @@ void launch_preference(const PairLoss& a, u64 rows, const i64* begin, u64 pairs,
     k_preference_lanes<8><<<blocks_for(pairs, 32), 256, 0, s>>>(a, rows, begin, pairs);
   } else if (average < 1024 && pairs >= 4 * kSMs) {
     k_preference_lanes<32><<<blocks_for(pairs, 8), 256, 0, s>>>(a, rows, begin, pairs);
+  } else if (pairs >= 1 && pairs <= kFewPairs && average >= kVeryLongRows && rows < (u64(kPieceRows) << 31)) {
+    const u32 pieces = u32((rows + kPieceRows - 1) / kPieceRows);
+    k_preference_pieces<<<pieces, 512, 0, s>>>(a, rows, begin, pairs);
+    after_launch("preference loss");
+    k_preference_settle<<<u32(pairs), 512, 0, s>>>(a, rows, begin);
+    after_launch("preference loss");
+    k_preference_spread<<<pieces, 512, 0, s>>>(a, rows, begin, pairs);
   } else {
-    // A block a pair; few pairs of very many rows: a cluster of larger blocks
-    // each, with more loads under way (one pair of 4M rows: 184 us by eight
-    // blocks of 512 threads, 84 by eight of 1024; 1000 pairs of 4000: 19 and 41).
+    // A block a pair; few pairs of many rows: a cluster of larger blocks
+    // each, with more loads under way (a cluster's 4M rows of one pair: 184 us
+    // by eight blocks of 512 threads, 84 by eight of 1024; 1000 pairs of 4000:
+    // 19 and 41).
     u32 blocks = 1;
     while (blocks < kPairCluster && pairs * blocks * 2 <= kSMs && average > 4096u * blocks) blocks *= 2;
     const bool large = average >= 32768;

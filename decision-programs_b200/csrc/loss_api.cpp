@@ -97,6 +97,11 @@ dp::PairLoss pair_args(const float* score, const float* ref, const float* weight
   need(rows == 0 || (score != nullptr && grad != nullptr), "score or gradient pointer is null");
   need(pairs == 0 || loss != nullptr, "loss pointer is null");
   check_aligned(score, ref, weight, loss, grad, hess);
+  // The outputs' places are written (partial sums too) while scores are read.
+  const Span z = span_of(score, rows, 1, 1, sizeof(float)), t = span_of(ref, rows, 1, 1, sizeof(float)),
+             o = span_of(grad, rows, 1, 1, sizeof(float)), h = span_of(hess, rows, 1, 1, sizeof(float));
+  need(!overlap(o, z) && !overlap(o, t), "the gradient overlaps the scores");
+  need(!overlap(h, z) && !overlap(h, t) && !overlap(h, o), "the curvature overlaps the scores or the gradient");
   dp::PairLoss a{};
   a.score = score;
   a.ref = ref;

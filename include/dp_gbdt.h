@@ -347,7 +347,8 @@ DP_API int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint
  * grad[rows] is its derivative by every score (all rows of an item share it),
  * hess[rows] (may be NULL) the second one, at least 1e-16; rows outside every
  * item get 0 (1e-16).  weight (per pair) NULL: 1; weight 0: the pair counts
- * for nothing, whatever its scores hold. */
+ * for nothing, whatever its scores hold.  Outputs that overlap the scores or
+ * each other are refused. */
 DP_API int dp_preference_loss(uint64_t rows, const int64_t* item_begin, uint64_t pairs, const float* score,
                               const float* ref_score, const float* weight, float beta, float smoothing, float* loss,
                               float* grad, float* hess, void* stream);

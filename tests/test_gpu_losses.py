@@ -349,14 +349,17 @@ def pair_bound(x, terms, w, beta, x_err):
 
 @pytest.mark.parametrize("use_ref", [False, True])
 @pytest.mark.parametrize("smoothing", [0.0, 0.1])
-@pytest.mark.parametrize("lengths", ["one", "short", "few", "uneven", "mixed", "long", "empty", "huge"])
+@pytest.mark.parametrize("lengths", ["one", "short", "few", "uneven", "mixed", "long", "empty", "huge", "ragged", "wide"])
 def test_preference_over_segments(dp, lengths, smoothing, use_ref):
     rng = np.random.default_rng(7)
-    items = {"one": 4000, "short": 600, "few": 9000, "uneven": 5000, "mixed": 200, "long": 6, "empty": 50, "huge": 2}[lengths]
+    items = {"one": 4000, "short": 600, "few": 9000, "uneven": 5000, "mixed": 200, "long": 6, "empty": 50, "huge": 2, "ragged": 10,
+             "wide": 6}[lengths]
     n = {"one": np.ones(items, int), "short": rng.integers(1, 9, items), "few": rng.integers(0, 9, items),
          "uneven": np.where(rng.random(items) < 0.002, 3000, rng.integers(0, 4, items)), "mixed": rng.integers(0, 700, items),
          "long": rng.integers(3000, 9000, items), "empty": rng.integers(0, 2, items),
-         "huge": np.array([300_001, 77_777])}[lengths]
+         "huge": np.array([300_001, 77_777]),
+         "wide": rng.integers(20_000, 60_000, items),
+         "ragged": np.array([0, 1_000_003, 3, 0, 150_000, 8191, 60_000, 250_001, 16_385, 0])}[lengths]
     lead, tail = (0, 0) if lengths == "one" else (3, 5)
     begin = lead + np.concatenate([[0], np.cumsum(n)])
     rows = int(begin[-1]) + tail

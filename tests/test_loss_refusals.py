@@ -127,3 +127,14 @@ def test_formulas_against_differences():
         up, down = ref64.pair_terms(x + step, smooth), ref64.pair_terms(x - step, smooth)
         assert np.allclose((up[0] - down[0]) / (2 * step), t[1], atol=1e-8)
         assert np.allclose((up[1] - down[1]) / (2 * step), t[2], atol=1e-8)
+
+
+def test_preference_outputs_may_not_overlap(dp):
+    call = lambda grad, hess=None, ref=None: refused(  # noqa: E731
+        dp, "dp_preference_loss", 8, None, 4, A, ref, None, 1.0, 0.0, A + 1024, grad, hess, None)
+    assert "gradient overlaps" in call(A)
+    assert "gradient overlaps" in call(A + 28)
+    assert "gradient overlaps" in call(A + 128, ref=A + 156)
+    assert "curvature overlaps" in call(A + 128, A)
+    assert "curvature overlaps" in call(A + 128, A + 128)
+    assert "curvature overlaps" in call(A + 128, A + 256, ref=A + 284)
