@@ -124,10 +124,13 @@ __global__ void __launch_bounds__(kPairBlock) k_preference_staged(PairLoss a, u6
   const u64 b0 = in ? clamp_row(begin[2 * p], rows) : 0, b1 = in ? clamp_row(begin[2 * p + 1], rows) : 0,
             b2 = in ? clamp_row(begin[2 * p + 2], rows) : 0;
   const float w = in && a.weight ? a.weight[p] : 1.f;
-  const bool fits = r1 >= r0 && r1 - r0 <= kStageRows;
-  const u32 n = fits ? u32(r1 - r0) : 0;
+  const bool room = r1 >= r0 && r1 - r0 <= kStageRows;
+  const u32 n = room ? u32(r1 - r0) : 0;
   for (u32 i = threadIdx.x; i < n; i += kPairBlock) stage[i] = gap(a, r0 + i);
-  __syncthreads();
+  // One answer for the block, since it decides on the barriers below: were the
+  // offsets written while the kernel runs, the results would be of no use, but
+  // every thread would still come to the same barriers.
+  const bool fits = __syncthreads_and(room);
   // (offsets out of order lead outside a pair's own rows, not outside the stage)
   auto local = [&](u64 b) { return b <= r0 ? 0u : u32(min(u64(n), b - r0)); };
   const u32 c0 = local(b0), c1 = local(b1), c2 = local(b2);
