@@ -2,6 +2,7 @@
 // include/dp_gbdt.h): argument checks on the host, then asynchronous launches
 // on the caller's stream.
 #include <cmath>
+#include <initializer_list>
 #include <memory>
 
 #include "../../include/dp_gbdt.h"
@@ -41,6 +42,16 @@ Span span_of(const void* p, u64 rows, u64 width, u64 stride, u64 size) {
   return rows && p ? Span{lo, lo + ((rows - 1) * stride + width) * size} : Span{};
 }
 bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+Span vector_of(const void* p, u64 n, u64 size = 4) { return span_of(p, n, 1, 1, size); }
+// Whether a vector touches an element of such rows (the gaps between rows are
+// no elements).
+bool touches_rows(const Span& v, const void* p, u64 rows, u64 width, u64 stride, u64 size) {
+  const Span all = span_of(p, rows, width, stride, size);
+  if (!overlap(v, all)) return false;
+  if (v.lo <= all.lo) return true;
+  const u64 row = (v.lo - all.lo) / (stride * size), at = (v.lo - all.lo) % (stride * size);
+  return at < width * size || (row + 1 < rows && all.lo + (row + 1) * stride * size < v.hi);
+}
 
 // A check whose message names an argument; it is put together only on failure.
 void need_of(bool ok, const char* what, const char* rule) {
@@ -90,18 +101,44 @@ dp::MarginGrad grad_of(const dp::Margins& m, void* grad, u64 grad_stride, float*
   return g;
 }
 
+// The vectors that a row call writes beside its gradient touch neither its
+// matrices nor each other, and the vectors that it reads only where they are
+// the same vector: a row is then read before it is written.
+void check_row_outputs(const dp::Margins& m, const dp::MarginGrad& g, std::initializer_list<Span> written,
+                       std::initializer_list<Span> read) {
+  const u64 size = dp::margin_bytes(m.dtype);
+  for (const Span* o = written.begin(); o != written.end(); ++o) {
+    need(!touches_rows(*o, m.z, m.rows, m.classes, m.stride, size), "an output vector overlaps the margins");
+    need(!touches_rows(*o, g.grad, m.rows, m.classes, g.grad_stride, size) &&
+             !touches_rows(*o, g.hess, m.rows, m.classes, g.hess_stride, sizeof(float)),
+         "an output vector overlaps the gradient or the curvature");
+    for (const Span* p = written.begin(); p != o; ++p) need(!overlap(*o, *p), "two output vectors overlap");
+    for (const Span& in : read)
+      need(!overlap(*o, in) || (o->lo == in.lo && o->hi == in.hi), "an output vector overlaps an input vector");
+  }
+  for (const Span& in : read)
+    need(!touches_rows(in, g.grad, m.rows, m.classes, g.grad_stride, size) &&
+             !touches_rows(in, g.hess, m.rows, m.classes, g.hess_stride, sizeof(float)),
+         "the gradient or the curvature overlaps an input vector");
+}
+
 dp::PairLoss pair_args(const float* score, const float* ref, const float* weight, float beta, float smoothing,
-                       float* loss, float* grad, float* hess, u64 rows, u64 pairs) {
+                       float* loss, float* grad, float* hess, u64 rows, u64 pairs, const Span& offsets = Span{}) {
   need(std::isfinite(beta) && beta > 0.f, "beta must be positive and finite");
   need(smoothing >= 0.f && smoothing <= 0.5f, "label smoothing must be in [0, 0.5]");
   need(rows == 0 || (score != nullptr && grad != nullptr), "score or gradient pointer is null");
   need(pairs == 0 || loss != nullptr, "loss pointer is null");
   check_aligned(score, ref, weight, loss, grad, hess);
-  // The outputs' places are written (partial sums too) while scores are read.
-  const Span z = span_of(score, rows, 1, 1, sizeof(float)), t = span_of(ref, rows, 1, 1, sizeof(float)),
-             o = span_of(grad, rows, 1, 1, sizeof(float)), h = span_of(hess, rows, 1, 1, sizeof(float));
+  // The outputs' places are written (partial sums too) while scores, weights
+  // and offsets are read.
+  const Span z = vector_of(score, rows), t = vector_of(ref, rows), o = vector_of(grad, rows), h = vector_of(hess, rows),
+             l = vector_of(loss, pairs), w = vector_of(weight, pairs);
   need(!overlap(o, z) && !overlap(o, t), "the gradient overlaps the scores");
   need(!overlap(h, z) && !overlap(h, t) && !overlap(h, o), "the curvature overlaps the scores or the gradient");
+  need(!overlap(l, z) && !overlap(l, t) && !overlap(l, o) && !overlap(l, h),
+       "the loss overlaps the scores, the gradient or the curvature");
+  for (const Span& out : {o, h, l})
+    need(!overlap(out, w) && !overlap(out, offsets), "an output overlaps the weights or the item offsets");
   dp::PairLoss a{};
   a.score = score;
   a.ref = ref;
@@ -131,6 +168,8 @@ int dp_log_prob(int32_t dtype, const void* margin, uint64_t rows, uint32_t class
     a.label = label;
     a.log_prob = log_prob;
     a.norm = reinterpret_cast<float2*>(norm);
+    check_row_outputs(m, a.out, {vector_of(log_prob, rows), vector_of(norm, rows, sizeof(float2))},
+                      {vector_of(label, rows)});
     dp::launch_rows(a, false, static_cast<cudaStream_t>(stream));
   });
 }
@@ -145,6 +184,8 @@ int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, uint32_t 
     need(reinterpret_cast<std::uintptr_t>(norm) % sizeof(float2) == 0, "norm pointer is not aligned to 8 bytes");
     check_aligned(label, weight);
     const dp::MarginGrad g = grad_of(m, grad, grad_stride, hess, hess_stride);
+    check_row_outputs(m, g, {},
+                      {vector_of(label, rows), vector_of(norm, rows, sizeof(float2)), vector_of(weight, rows)});
     dp::launch_grad(dp::GradArgs{m, label, reinterpret_cast<const float2*>(norm), weight, g},
                     static_cast<cudaStream_t>(stream));
   });
@@ -170,6 +211,9 @@ int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t cl
     a.loss = loss;
     a.log_prob = log_prob;
     a.out = grad_of(m, grad, grad_stride, hess, hess_stride);
+    check_row_outputs(m, a.out, {vector_of(loss, rows), vector_of(log_prob, rows)},
+                      {vector_of(label, rows), vector_of(old_log_prob, rows), vector_of(ref_log_prob, rows),
+                       vector_of(advantage, rows), vector_of(weight, rows)});
     dp::PolicyRows& p = a.policy;
     p.old_log_prob = old_log_prob;
     p.ref_log_prob = ref_log_prob;
@@ -190,7 +234,8 @@ int dp_preference_loss(uint64_t rows, const int64_t* item_begin, uint64_t pairs,
     check_aligned(item_begin);
     need(item_begin != nullptr || rows >= 2 * pairs, "without item offsets every pair needs two rows");
     const dp::PairLoss a =
-        pair_args(score, ref_score, weight, beta, smoothing, loss, grad, hess, rows, pairs);
+        pair_args(score, ref_score, weight, beta, smoothing, loss, grad, hess, rows, pairs,
+                  item_begin ? vector_of(item_begin, 2 * pairs + 1, sizeof(int64_t)) : Span{});
     dp::launch_preference(a, rows, item_begin, pairs, static_cast<cudaStream_t>(stream));
   });
 }

@@ -309,7 +309,10 @@ DP_API int dp_eval_splits(const int64_t* hist, int32_t nnodes, uint32_t features
  *  - margins of -inf are masked classes of probability 0.  A row that masks
  *    every class has log-probability -inf, loss 0 and a zero gradient.
  *  - NaN or +inf in a row that is not skipped makes that row's results NaN,
- *    and no other's. */
+ *    and no other's.
+ * Outputs may not overlap the margins, each other or an input, with two
+ * exceptions: grad may be margin itself (same row stride), and a vector of
+ * [rows] that is written may be one that is read (same pointer). */
 
 /* log_prob[rows] = log softmax(margin)[label], and norm[rows][2] = (maximum,
  * log of the sum of exp(margin - maximum)), which dp_log_prob_grad reads. */
@@ -319,8 +322,7 @@ DP_API int dp_log_prob(int32_t dtype, const void* margin, uint64_t rows, uint32_
  * ([k == label] - p_k), weight being the derivative of a loss by log_prob[r];
  * hess (fp32, may be NULL) = |weight[r]| * max(2 p_k (1 - p_k), 1e-16), the
  * softmax objective's diagonal form.  weight 0: the row's outputs are 0,
- * whatever its margins hold.  grad may be margin itself (same row stride);
- * other overlaps are refused. */
+ * whatever its margins hold. */
 DP_API int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
                             const int32_t* label, const float* norm, const float* weight, void* grad,
                             uint64_t grad_stride, float* hess, uint64_t hess_stride, void* stream);
@@ -347,8 +349,8 @@ DP_API int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint
  * grad[rows] is its derivative by every score (all rows of an item share it),
  * hess[rows] (may be NULL) the second one, at least 1e-16; rows outside every
  * item get 0 (1e-16).  weight (per pair) NULL: 1; weight 0: the pair counts
- * for nothing, whatever its scores hold.  Outputs that overlap the scores or
- * each other are refused. */
+ * for nothing, whatever its scores hold.  Outputs that overlap each other,
+ * the scores, the weights or the offsets are refused. */
 DP_API int dp_preference_loss(uint64_t rows, const int64_t* item_begin, uint64_t pairs, const float* score,
                               const float* ref_score, const float* weight, float beta, float smoothing, float* loss,
                               float* grad, float* hess, void* stream);
