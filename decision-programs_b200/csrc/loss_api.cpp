@@ -216,7 +216,7 @@ int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t cl
                        vector_of(advantage, rows), vector_of(weight, rows)});
     dp::PolicyRows& p = a.policy;
     p.old_log_prob = old_log_prob;
-    p.ref_log_prob = ref_log_prob;
+    p.ref_log_prob = kl != 0.f ? ref_log_prob : nullptr;  // (0 times an infinite term would be NaN)
     p.advantage = advantage;
     p.weight = weight;
     p.clip_low = clip_low;

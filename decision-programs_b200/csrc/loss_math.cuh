@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
+
 #include "loss.h"
 
 namespace dp {
@@ -61,15 +63,27 @@ struct RowScalars {
   float zy = 0.f, old = 0.f, ref = 0.f, adv = 0.f, w = 1.f;
 };
 
+// The lesser of two numbers, a NaN where there is one.
+__device__ __forceinline__ float least_of(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+constexpr float kMostSlope = 0x1p126f;
+
 // Clipped policy loss of a row and its derivative by the log-probability:
 // L = w (-min(r A, clamp(r, 1 - lo, 1 + hi) A) + kl (e^d - d - 1)),
-// r = exp(l - old), d = ref - l.  Comparisons keep a NaN ratio NaN.
+// r = exp(l - old), d = ref - l.  Comparisons keep a NaN ratio NaN.  A masked
+// class that was chosen has l = -inf, so that r = 0 and d is infinite.  Ratios
+// past fp32's range are held to its largest number (no advantage makes nothing
+// of them), and the derivative to kMostSlope in size: an infinite one would make
+// NaN of the classes of probability 0, and twice kMostSlope is still finite.
 __device__ __forceinline__ float policy_row(const PolicyRows& p, const RowScalars& x, float l, float& loss) {
   if (x.w == 0.f) {
     loss = 0.f;
     return 0.f;
   }
-  const float ratio = exp_fast(l - x.old), adv = x.adv;
+  const float ratio = least_of(exp_fast(l - x.old), FLT_MAX), adv = x.adv;
   const float low = 1.f - p.clip_low, high = 1.f + p.clip_high;
   const float held = ratio < low ? low : (ratio > high ? high : ratio);
   const float s1 = ratio * adv, s2 = held * adv;
@@ -88,12 +102,13 @@ __device__ __forceinline__ float policy_row(const PolicyRows& p, const RowScalar
     t = fmaf(t, d, 1.f / 6.f);
     t = fmaf(t, d, 0.5f);
     const bool near = fabsf(d) < 0.5f;
-    const float e = exp_fast(d), over = near ? t * d * d : (e - d) - 1.f;
+    // (an infinite d: e^d - d is e^d)
+    const float e = exp_fast(d), over = near ? t * d * d : (e - fminf(d, FLT_MAX)) - 1.f;
     v = v + p.kl * over;
-    c = c - p.kl * (near ? over + d : e - 1.f);
+    c = c - least_of(p.kl * (near ? over + d : e - 1.f), kMostSlope);
   }
   loss = x.w * v;
-  return x.w * c;
+  return -least_of(-least_of(x.w * c, kMostSlope), kMostSlope);
 }
 
 // Gradient and curvature of c * log p(label) by one margin of probability p.

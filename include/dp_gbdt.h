@@ -306,8 +306,9 @@ DP_API int dp_eval_splits(const int64_t* hist, int32_t nnodes, uint32_t features
  * exponentials are fp32; a gradient is rounded to `dtype` once.
  *  - label (int32) outside [0, classes): the row is skipped: whatever its
  *    margins hold, its outputs and its gradient row are 0.
- *  - margins of -inf are masked classes of probability 0.  A row that masks
- *    every class has log-probability -inf, loss 0 and a zero gradient.
+ *  - margins of -inf are masked classes of probability 0 (chosen: of
+ *    log-probability -inf).  A row that masks every class has log-probability
+ *    -inf, loss 0 and a zero gradient.
  *  - NaN or +inf in a row that is not skipped makes that row's results NaN,
  *    and no other's.
  * Outputs may not overlap the margins, each other or an input, with two
@@ -330,10 +331,15 @@ DP_API int dp_log_prob_grad(int32_t dtype, const void* margin, uint64_t rows, ui
  * l = log softmax(margin)[label], r = exp(l - old_log_prob), d = ref_log_prob - l,
  * loss[rows] = weight * (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
  *                        + kl (exp(d) - d - 1)),
- * A the advantage.  ref_log_prob NULL: no KL term; weight NULL: 1; weight 0:
- * loss and gradient row are 0 whatever the row holds.  log_prob[rows]
+ * A the advantage.  ref_log_prob NULL or kl 0: no KL term; weight NULL: 1;
+ * weight 0: loss and gradient row are 0 whatever the row holds.  log_prob[rows]
  * receives l.  grad / hess as in dp_log_prob_grad with the loss's derivative
- * by l for its weight; grad NULL: the forward pass alone. */
+ * by l for its weight; grad NULL: the forward pass alone.  Where r A or exp(d)
+ * passes fp32's range (a masked class chosen, with a KL term) the loss is
+ * infinite (r itself counts as 3.4e38 at most), and its derivative by l a large
+ * finite number, 2^126 at most, so that classes of probability 0 keep a gradient
+ * of 0.  l and old_log_prob (or, with a KL term, ref_log_prob) that are both
+ * -inf have no ratio: the row is NaN. */
 DP_API int dp_policy_loss(int32_t dtype, const void* margin, uint64_t rows, uint32_t classes, uint64_t row_stride,
                           const int32_t* label, const float* old_log_prob, const float* ref_log_prob,
                           const float* advantage, const float* weight, float clip_low, float clip_high, float kl,

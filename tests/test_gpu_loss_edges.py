@@ -53,3 +53,96 @@ def test_vectors_in_each_others_place(dp, rows, classes):
                                      logp.data_ptr(), grad.data_ptr(), classes, None, 0,
                                      torch.cuda.current_stream().cuda_stream))
     assert torch.equal(loss, want.loss) and torch.equal(logp, want.log_prob) and torch.equal(grad, want.grad)
+
+
+def formula_rows(z64, y, c):
+    """Gradient and curvature of sum c * log p(y), the coefficient's size finite."""
+    p = np.exp(z64 - z64.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    hit = np.zeros_like(p)
+    hit[np.arange(len(y)), y] = 1.0
+    return c[:, None] * (hit - p), np.abs(c)[:, None] * np.maximum(2 * p * (1 - p), 1e-16)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("classes", [4, 6, 40, 90, 1500, 20_011, 140_001])
+def test_chosen_classes_that_are_masked_and_ratios_past_the_range(dp, dtype, classes):
+    """Rows whose chosen class is masked (kinds 0 and 1), whose ratio or whose
+    reference's lead passes fp32's range (2 and 3), and plain ones (4), with
+    advantages of each sign and none."""
+    rows = 30
+    rng = np.random.default_rng(classes)
+    y = rng.integers(0, classes, rows).astype(np.int32)
+    kind, adv = np.arange(rows) % 5, np.tile(np.repeat([1.5, -2.0, 0.0], 5), 2).astype(np.float32)
+    z = torch.from_numpy(rng.standard_normal((rows, classes)).astype(np.float32)).to(getattr(torch, dtype)).cuda()
+    z64 = z.double().cpu().numpy()
+    for r in range(rows):
+        if kind[r] in (0, 1):
+            z64[r, y[r]] = -np.inf
+        if classes > 4:  # other masks beside the chosen class
+            z64[r, (y[r] + 1) % classes] = -np.inf
+    z.copy_(torch.from_numpy(z64).to(z.dtype))
+    up = lambda v: torch.from_numpy(np.asarray(v, np.float32)).cuda()  # noqa: E731
+    yd = torch.from_numpy(y).cuda()
+    with np.errstate(divide="ignore"):
+        logp64 = (z64 - z64.max(1, keepdims=True) - np.log(np.exp(z64 - z64.max(1, keepdims=True)).sum(1, keepdims=True)))
+    logp64 = logp64[np.arange(rows), y]
+    # p is off by the sum's and the exponential's error, below 2^-12 at this many
+    # classes; a coefficient by log p's, below 1e-4; a gradient is rounded to its type
+    step = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}[dtype]
+
+    def check(g, h, c):
+        g, h = g.double().cpu().numpy(), h.double().cpu().numpy()
+        want_g, want_h = formula_rows(z64, y, c)
+        size = np.abs(c)[:, None]
+        past = np.abs(want_g) > (65520 if dtype == "float16" else 3e38)
+        assert not np.isnan(g).any() and not np.isnan(h).any()
+        assert np.array_equal(g[past], np.sign(want_g[past]) * np.inf)
+        off = np.abs(np.where(past, 0.0, g) - np.where(past, 0.0, want_g))
+        assert np.all(off <= (step + 2.0 ** -12) * np.abs(want_g) + 1e-4 * size + 2.0 ** -24)
+        assert np.all(np.abs(h - want_h) <= 2.0 ** -11 * want_h + 1e-4 * size + 1e-30)
+        assert np.all(g[hidden] == 0)
+    hidden = (z64 == -np.inf) & (np.arange(classes)[None] != y[:, None])
+
+    def large(r, at, sign):
+        """The finite slope of rows where the formula's is past the range, from the curvature's floor and largest entry."""
+        _, unit = formula_rows(z64, y, np.ones(rows))
+        top = unit.argmax(1)
+        size = (r.hess.double().cpu().numpy()[np.arange(rows), top] / unit[np.arange(rows), top])[at]
+        assert np.all((size >= 2.0 ** 120) & (size <= 2.0 ** 126 * 1.001))
+        return sign * size
+
+    logp, norm = dp.log_prob(z, yd)
+    assert np.array_equal(logp.cpu().numpy() == -np.inf, (kind == 0) | (kind == 1))
+    seen = np.isfinite(logp64)
+    assert np.allclose(logp.cpu().numpy()[seen], logp64[seen], rtol=0, atol=2e-4)
+    c = rng.standard_normal(rows)
+    check(*dp.log_prob_grad(z, yd, norm, up(c), hess=True), np.float32(c).astype(np.float64))
+
+    base = np.where(seen, logp64, -3.0)
+    old, ref = base - np.where(kind == 2, 100.0, 0.1), base + np.where(kind == 3, 100.0, 0.2)
+    call = lambda **kw: dp.policy_loss(z, yd, up(old), up(adv), weight=up(np.full(rows, 0.5)), clip=(0.2, 0.3),  # noqa: E731
+                                       hess=True, **kw)
+    free = call()
+    ratio = np.where(seen, np.exp(np.minimum(np.where(seen, logp64, 0) - old, 99.0)), 0.0)
+    s1, s2 = ratio * adv, np.clip(ratio, 0.8, 1.3) * adv
+    loss, slope = -0.5 * np.minimum(s1, s2), 0.5 * np.where(s1 <= s2, -s1, 0.0)
+    wild = (kind == 2) & (adv < 0)  # e^100 passes fp32's range
+    got = free.loss.double().cpu().numpy()
+    assert np.all(got[wild] == np.inf) and np.allclose(got[~wild], loss[~wild], rtol=1e-3, atol=1e-6)
+    slope[wild] = large(free, wild, 1)
+    # kl 0: the reference's log-probabilities, infinite lead or not, count for nothing
+    for other in (call(ref_log_prob=up(ref)), call(ref_log_prob=up(np.full(rows, -np.inf)))):
+        assert all(torch.equal(u, v) for u, v in zip(other, free))
+    kl = call(ref_log_prob=up(ref), kl=0.1)
+    far = (kind == 3) | ~seen
+    got = kl.loss.double().cpu().numpy()
+    with np.errstate(over="ignore", invalid="ignore"):
+        d = np.where(far, 0.0, ref - np.where(seen, logp64, 0.0))
+        over = 0.5 * 0.1 * (np.expm1(d) - d)
+    tame = ~(far | wild)
+    assert np.all(got[~tame] == np.inf) and np.allclose(got[tame], (loss + over)[tame], rtol=1e-3, atol=1e-6)
+    lead = slope - 0.5 * 0.1 * np.expm1(d)
+    lead[far], lead[wild] = large(kl, far, -1), large(kl, wild, 1)
+    check(free.grad, free.hess, slope)
+    check(kl.grad, kl.hess, lead)
