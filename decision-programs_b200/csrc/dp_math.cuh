@@ -57,12 +57,13 @@ DP_HD double dp_exp(double x) {
   return ldexp(p, int(k));
 }
 
-// Power-of-two scale s with |v * s| < 2^bits for every |v| <= vmax.
+// Power-of-two scale s with |v * s| < 2^bits for every |v| <= vmax, vmax any
+// finite number (below 2^-100 with fewer bits, so that s stays finite).
 DP_HD float quant_scale(float vmax, int bits) {
   if (!(vmax > 0.0f)) return 1.0f;
   int e = 0;
   frexpf(vmax, &e);
-  e = e < -100 ? -100 : (e > 100 ? 100 : e);
+  e = e < -100 ? -100 : e;
   return ldexpf(1.0f, bits - e);
 }
 

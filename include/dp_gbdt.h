@@ -92,7 +92,10 @@ DP_API int XGBoosterUpdateOneIter(BoosterHandle handle, int iter, DMatrixHandle 
  * labels.  Waits for the device's earlier work, and is synchronous like
  * XGBoosterUpdateOneIter; rounds of both kinds may alternate.  Values that are
  * not finite and negative curvatures are refused and leave the model as it
- * was.  XGBoost C API function; the reference does not bind it. */
+ * was.  Sums are exact over values rounded to steps of 2^-17 to 2^-16 of the
+ * output's largest |grad| of the round (2^-18 to 2^-17 of its largest curvature):
+ * rows whose gradients are 2^18 times smaller than another's count as 0.
+ * XGBoost C API function; the reference does not bind it. */
 DP_API int XGBoosterTrainOneIter(BoosterHandle handle, DMatrixHandle dtrain, int iter, const char* grad,
                                  const char* hess);
 

@@ -380,12 +380,13 @@ void gradients(int objective, int K, const float* margin, const float* label, ui
   });
 }
 
-// Power-of-two quantiser scale: |v*s| < 2^bits for all |v| <= vmax.
+// Power-of-two quantiser scale: |v*s| < 2^bits for all |v| <= vmax, any finite
+// vmax (below 2^-100 with fewer bits, so that s stays finite).
 float quant_scale(float vmax, int bits) {
   if (!(vmax > 0.0f)) return 1.0f;
   int e = 0;
   std::frexp(vmax, &e);
-  e = std::max(-100, std::min(100, e));
+  e = std::max(-100, e);
   return std::ldexp(1.0f, bits - e);
 }
 
