@@ -110,14 +110,91 @@ __device__ __forceinline__ void fill_outside(const PairLoss& a, u64 rows, const 
   span_fill(a, last, rows, me, step, 0.f, item_hess(0.f));
 }
 
+// Sums of v over the block's threads, the same in each of them.
+template <int kWarps>
+__device__ __forceinline__ float2 block_sums(float2 v, float2* part) {
+  v.x = lanes_sum<32>(v.x);
+  v.y = lanes_sum<32>(v.y);
+  __syncthreads();  // (the last call's parts have been read)
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[threadIdx.x & (kWarps - 1)];
+  return make_float2(lanes_sum<kWarps>(v.x), lanes_sum<kWarps>(v.y));
+}
+
+// Pairs far longer than the others of their call, which one thread or a few
+// lanes would take while the device waits, and sum in long chains: the whole
+// block takes them one after another (100,000 short pairs and one item of a
+// million rows: 258 us, by one thread 16.9 ms).  What only such pairs need is
+// kept out of the kernels' own code, whose registers it would take.
+struct LongPair {
+  u64 p, b0, b1, b2;
+};
+// Rows that one lane of a pair takes, 64 loads of four rows one after another.
+constexpr u64 kLaneRows = 256;
+template <int kThreads>
+__device__ __forceinline__ void take_long_pairs(const PairLoss& a, const LongPair* list, u32 n) {
+  __shared__ float2 part[kThreads / 32];
+  for (u32 i = 0; i < n; ++i) {
+    const LongPair x = list[i];
+    const float2 s = block_sums<kThreads / 32>(make_float2(span_sum<8>(a, x.b0, x.b1, threadIdx.x, kThreads),
+                                                           span_sum<8>(a, x.b1, x.b2, threadIdx.x, kThreads)), part);
+    const PairResult o = pair_result(a, s.x - s.y, a.weight ? a.weight[x.p] : 1.f);
+    const float h = item_hess(o.h);
+    if (threadIdx.x == 0) a.loss[x.p] = o.loss;
+    span_fill(a, x.b0, x.b1, threadIdx.x, kThreads, o.q, h);
+    span_fill(a, x.b1, x.b2, threadIdx.x, kThreads, -o.q, h);
+  }
+}
+
 // Items of a few rows: a block stages the rows of 256 pairs in shared memory,
 // a thread takes a pair, and the gradients go out as the scores came in, in
 // whole lines.  (4M rows in 1M pairs: 118 us by 8 lanes a pair.)  Blocks whose
-// rows do not fit take their pairs one thread each from memory.
+// rows do not fit take their pairs from memory, each by a thread, a warp or the
+// block as its length asks.
 constexpr u32 kPairBlock = 256, kStageRows = 4096;
-__global__ void __launch_bounds__(kPairBlock) k_preference_staged(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
-  __shared__ float stage[kStageRows];
+__device__ __noinline__ void take_unstaged_pairs(const PairLoss& call, u64 rows, const i64* begin, u64 pairs, LongPair* list, u32* longs) {
+  const PairLoss a = call;
+  const u64 p = u64(blockIdx.x) * kPairBlock + threadIdx.x;
+  const bool in = p < pairs;
+  const u64 b0 = in ? clamp_row(begin[2 * p], rows) : 0, b1 = in ? clamp_row(begin[2 * p + 1], rows) : 0,
+            b2 = in ? clamp_row(begin[2 * p + 2], rows) : 0, n = b2 - b0;
+  const float w = in && a.weight ? a.weight[p] : 1.f;
+  if (threadIdx.x == 0) *longs = 0;
+  __syncthreads();
+  // (a warp takes its longer pairs one after another; many of them, unless very
+  // long, go by a thread each: 300,000 pairs of lognormal lengths in ascending
+  // order 109 us, without 118)
+  const bool many = __popc(__ballot_sync(0xffffffffu, n > kLaneRows)) > 12;
+  const u64 alone = many ? 4 * kLaneRows : kLaneRows;
+  if (in && n <= alone) {
+    const PairResult o = pair_result(a, span_sum<4>(a, b0, b1, 0, 1) - span_sum<4>(a, b1, b2, 0, 1), w);
+    const float h = item_hess(o.h);
+    a.loss[p] = o.loss;
+    span_fill(a, b0, b1, 0, 1, o.q, h);
+    span_fill(a, b1, b2, 0, 1, -o.q, h);
+  }
+  const bool whole = n > 32 * kLaneRows;
+  if (whole) list[atomicAdd(longs, 1u)] = LongPair{p, b0, b1, b2};
+  const u32 lane = threadIdx.x & 31;
+  for (u32 todo = __ballot_sync(0xffffffffu, n > alone && !whole); todo; todo &= todo - 1) {
+    const int from = __ffs(int(todo)) - 1;
+    const u64 c0 = __shfl_sync(0xffffffffu, b0, from), c1 = __shfl_sync(0xffffffffu, b1, from),
+              c2 = __shfl_sync(0xffffffffu, b2, from);
+    const float sa = lanes_sum<32>(span_sum<8>(a, c0, c1, lane, 32)), sb = lanes_sum<32>(span_sum<8>(a, c1, c2, lane, 32));
+    const PairResult o = pair_result(a, sa - sb, __shfl_sync(0xffffffffu, w, from));
+    const float h = item_hess(o.h);
+    if (int(lane) == from) a.loss[p] = o.loss;
+    span_fill(a, c0, c1, lane, 32, o.q, h);
+    span_fill(a, c1, c2, lane, 32, -o.q, h);
+  }
+  __syncthreads();
+  take_long_pairs<kPairBlock>(a, list, *longs);
+}
+__global__ void __launch_bounds__(kPairBlock, 6) k_preference_staged(const __grid_constant__ PairLoss a, u64 rows, const i64* begin, u64 pairs) {
+  __shared__ __align__(16) float stage[kStageRows];
   __shared__ float stage_h[kStageRows];
+  __shared__ u32 longs;
   const u64 p0 = u64(blockIdx.x) * kPairBlock, p1 = min(pairs, p0 + kPairBlock), p = p0 + threadIdx.x;
   const u64 r0 = clamp_row(begin[2 * p0], rows), r1 = clamp_row(begin[2 * p1], rows);
   const bool in = p < p1;
@@ -130,22 +207,16 @@ __global__ void __launch_bounds__(kPairBlock) k_preference_staged(PairLoss a, u6
   // One answer for the block, since it decides on the barriers below: were the
   // offsets written while the kernel runs, the results would be of no use, but
   // every thread would still come to the same barriers.
-  const bool fits = __syncthreads_and(room);
-  // (offsets out of order lead outside a pair's own rows, not outside the stage)
-  auto local = [&](u64 b) { return b <= r0 ? 0u : u32(min(u64(n), b - r0)); };
-  const u32 c0 = local(b0), c1 = local(b1), c2 = local(b2);
-  float sa = 0.f, sb = 0.f;
-  if (fits) {
+  if (__syncthreads_and(room)) {
+    // (offsets out of order lead outside a pair's own rows, not outside the stage)
+    auto local = [&](u64 b) { return b <= r0 ? 0u : u32(min(u64(n), b - r0)); };
+    const u32 c0 = local(b0), c1 = local(b1), c2 = local(b2);
+    float sa = 0.f, sb = 0.f;
     for (u32 i = c0; i < c1; ++i) sa += stage[i];
     for (u32 i = c1; i < c2; ++i) sb += stage[i];
-  } else {
-    sa = span_sum<4>(a, b0, b1, 0, 1);
-    sb = span_sum<4>(a, b1, b2, 0, 1);
-  }
-  const PairResult o = pair_result(a, sa - sb, w);
-  const float h = item_hess(o.h);
-  if (in) a.loss[p] = o.loss;
-  if (fits) {
+    const PairResult o = pair_result(a, sa - sb, w);
+    const float h = item_hess(o.h);
+    if (in) a.loss[p] = o.loss;
     __syncthreads();  // (every sum has been taken)
     if (in) {
       for (u32 i = c0; i < c1; ++i) { stage[i] = o.q; stage_h[i] = h; }
@@ -156,25 +227,56 @@ __global__ void __launch_bounds__(kPairBlock) k_preference_staged(PairLoss a, u6
       a.grad[r0 + i] = stage[i];
       if (a.hess) a.hess[r0 + i] = stage_h[i];
     }
-  } else if (in) {
-    span_fill(a, b0, b1, 0, 1, o.q, h);
-    span_fill(a, b1, b2, 0, 1, -o.q, h);
+  } else {
+    static_assert(sizeof stage >= kPairBlock * sizeof(LongPair), "the stage holds a block's long pairs");
+    take_unstaged_pairs(a, rows, begin, pairs, reinterpret_cast<LongPair*>(stage), &longs);
   }
   fill_outside(a, rows, begin, pairs);
 }
 
-// Short items: G lanes a pair.
+// The pairs that the lanes of a block have left, looked for N at a time.
+template <int N, int G>
+__device__ __noinline__ void take_left_pairs(const PairLoss& call, u64 rows, const i64* begin, u64 pairs, LongPair* list, u32* longs) {
+  const PairLoss a = call;
+  for (u64 p0 = u64(blockIdx.x) * N; p0 < pairs; p0 += u64(gridDim.x) * N) {
+    const u64 p = p0 + threadIdx.x;
+    if (threadIdx.x == 0) *longs = 0;
+    __syncthreads();
+    if (threadIdx.x < N && p < pairs) {
+      const LongPair x{p, clamp_row(begin[2 * p], rows), clamp_row(begin[2 * p + 1], rows), clamp_row(begin[2 * p + 2], rows)};
+      if (x.b2 - x.b0 > G * kLaneRows) list[atomicAdd(longs, 1u)] = x;
+    }
+    __syncthreads();
+    take_long_pairs<256>(a, list, *longs);
+    __syncthreads();  // (the list has been read)
+  }
+}
+
+// Short items: G lanes a pair; a pair past kLaneRows rows a lane waits for the
+// block (4M rows in 20,000 even pairs 20.8 us, by lanes alone 19.8; 3000 pairs of
+// 300 rows and an item of 2^20 rows 257 us, by lanes alone 1605).
 template <int G>
-__global__ void __launch_bounds__(256) k_preference_lanes(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
+__global__ void __launch_bounds__(256, 6) k_preference_lanes(const __grid_constant__ PairLoss a, u64 rows, const i64* begin, u64 pairs) {
+  __shared__ LongPair list[256 / G];
+  __shared__ u32 longs;
   const u32 lane = threadIdx.x % G;
-  const u64 per_block = 256 / G, step = u64(gridDim.x) * per_block;
-  for (u64 p0 = u64(blockIdx.x) * per_block; p0 < pairs; p0 += step) {
+  const u64 per_block = 256 / G, step = u64(gridDim.x) * per_block, first = u64(blockIdx.x) * per_block;
+  bool left = false;
+  for (u64 p0 = first; p0 < pairs; p0 += step) {
     const u64 p = p0 + threadIdx.x / G;
     const bool in = p < pairs;  // (the lanes of a warp sum together)
     const u64 b0 = in ? clamp_row(begin[2 * p], rows) : 0, b1 = in ? clamp_row(begin[2 * p + 1], rows) : 0,
               b2 = in ? clamp_row(begin[2 * p + 2], rows) : 0;
-    const float sa = lanes_sum<G>(span_sum<4>(a, b0, b1, lane, G)), sb = lanes_sum<G>(span_sum<4>(a, b1, b2, lane, G));
-    if (!in) continue;
+    const bool take = b2 - b0 <= G * kLaneRows;
+    left |= !take;
+    float sa = 0.f, sb = 0.f;
+    if (take) {
+      sa = span_sum<4>(a, b0, b1, lane, G);
+      sb = span_sum<4>(a, b1, b2, lane, G);
+    }
+    sa = lanes_sum<G>(sa);
+    sb = lanes_sum<G>(sb);
+    if (!in || !take) continue;
     const PairResult o = pair_result(a, sa - sb, a.weight ? a.weight[p] : 1.f);
     const float h = item_hess(o.h);
     if (lane == 0) a.loss[p] = o.loss;
@@ -182,6 +284,7 @@ __global__ void __launch_bounds__(256) k_preference_lanes(PairLoss a, u64 rows, 
     span_fill(a, b1, b2, lane, G, -o.q, h);
   }
   fill_outside(a, rows, begin, pairs);
+  if (__syncthreads_or(left)) take_left_pairs<256 / G, G>(a, rows, begin, pairs, list, &longs);
 }
 
 // Long items: a block, or a cluster of blocks, a pair.
@@ -255,17 +358,6 @@ struct PairSpan {
 __device__ __forceinline__ void read_offsets(u64* offset, const i64* begin, u64 pairs, u64 rows) {
   for (u64 i = threadIdx.x; i <= 2 * pairs; i += blockDim.x) offset[i] = clamp_row(begin[i], rows);
   __syncthreads();
-}
-// Sums of v over the block's threads, the same in each of them.
-template <int kWarps>
-__device__ __forceinline__ float2 block_sums(float2 v, float2* part) {
-  v.x = lanes_sum<32>(v.x);
-  v.y = lanes_sum<32>(v.y);
-  __syncthreads();  // (the last call's parts have been read)
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = part[threadIdx.x & (kWarps - 1)];
-  return make_float2(lanes_sum<kWarps>(v.x), lanes_sum<kWarps>(v.y));
 }
 __global__ void __launch_bounds__(512) k_preference_pieces(PairLoss a, u64 rows, const i64* begin, u64 pairs) {
   __shared__ float2 part[16];

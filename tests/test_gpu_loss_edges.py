@@ -146,3 +146,45 @@ def test_chosen_classes_that_are_masked_and_ratios_past_the_range(dp, dtype, cla
     lead[far], lead[wild] = large(kl, far, -1), large(kl, wild, 1)
     check(free.grad, free.hess, slope)
     check(kl.grad, kl.hess, lead)
+
+
+def exact_items(items, lengths):
+    """Scores whose sums are exact by trees and by chains of up to 4095 terms, and
+    not by longer chains: 4097 in each row of the long items (whose lengths are
+    powers of two), small integers in the others."""
+    rng = np.random.default_rng(items)
+    score = rng.integers(-2, 3, int(lengths.sum())).astype(np.float32)
+    begin = offsets(lengths)
+    for i in np.flatnonzero(lengths >= 1 << 13):
+        score[begin[i]:begin[i + 1]] = 4097.0
+    return score, begin
+
+
+@pytest.mark.parametrize("use_ref", [False, True])
+@pytest.mark.parametrize("pairs,short", [(100_000, 2), (20_000, 10), (40_000, 15), (3000, 150)])
+def test_very_long_items_among_short_ones(dp, pairs, short, use_ref):
+    """A call of short items has items of 2^13, 2^14 and 2^20 rows: their sums are as
+    exact as those of a call of long items, in any kernel of short ones."""
+    lengths = np.full(2 * pairs, short)
+    lengths[[7, 2 * pairs // 3 | 1, 2 * pairs - 4]] = 1 << 13, 1 << 20, 1 << 14
+    lengths[600:606] = 0, 700, 700, 0, 5000, 3  # and some in between
+    lengths[::17] = 0
+    score, begin = exact_items(pairs, lengths)
+    refs = np.where(np.abs(score) > 4000, 0.0, -1.0).astype(np.float32) if use_ref else None
+    gap = score.astype(np.float64) - (refs if use_ref else 0.0)
+    run = np.concatenate([[0.0], np.cumsum(gap)])
+    total = run[begin[1:]] - run[begin[:-1]]
+    beta = float(np.float32(2.0 ** -31))
+    x = beta * (total[0::2] - total[1::2])  # of size 2 for the longest item
+    assert 1.9 < np.abs(x).max() < 2.1
+    up = lambda v: None if v is None else torch.from_numpy(v).cuda()  # noqa: E731
+    r = dp.preference_loss(up(score), ref_score=up(refs), item_begin=up(begin), beta=beta, hess=True)
+    # sums and their difference are exact: x, softplus and the sigmoids are rounded a few times each
+    e = 2.0 ** -24
+    loss, down = np.logaddexp(0, -x), 1 / (1 + np.exp(x))
+    assert np.all(np.abs(r.loss.double().cpu().numpy() - loss) <= 16 * e * loss + 4 * e * np.abs(x) + 4 * e)
+    q = np.repeat(np.stack([-beta * down, beta * down], 1).reshape(-1), lengths)
+    h = np.repeat(np.maximum(beta * beta * down * (1 - down), 1e-16).repeat(2), lengths)
+    off = 16 * e + 4 * e * np.repeat(np.abs(x).repeat(2), lengths)
+    assert np.all(np.abs(r.grad.double().cpu().numpy() - q) <= beta * off)
+    assert np.all(np.abs(r.hess.double().cpu().numpy() - h) <= beta * beta * off + 1e-22)
