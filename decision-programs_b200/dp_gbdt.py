@@ -458,6 +458,9 @@ class CsvTable:
 # ---- losses that learn from choices ------------------------------------------
 # Each call runs on the current torch stream of its tensors' device and returns
 # new tensors; nothing waits for the GPU (PreferencePairs' construction aside).
+# Results are detached: autograd records none of these calls, also where a
+# tensor requires a gradient; the gradients returned are what a caller hands on
+# (margin.backward(grad), or Booster.boost).
 
 class PolicyLoss(NamedTuple):
     """loss and log_prob [R] fp32; grad [R, K] of the margins' type and hess
@@ -537,8 +540,8 @@ def _grad_out(margin, grad, hess):
     if grad is None or grad is True:
         grad = torch.empty_like(margin)  # (margins whose rows lie apart: without the gaps)
     else:
-        _need(grad.shape == margin.shape and grad.dtype == margin.dtype and grad.device == margin.device,
-              "grad must have the margins' shape, type and device")
+        _need(isinstance(grad, torch.Tensor) and grad.shape == margin.shape and grad.dtype == margin.dtype and
+              grad.device == margin.device, "grad must be a tensor of the margins' shape, type and device")
     if not hess:
         return grad, None, (*_rows_of(grad, "grad"), None, 0)
     hess = torch.empty_like(margin, dtype=torch.float32)
@@ -549,7 +552,8 @@ def log_prob(margin, label):
     """log softmax(margin)[label] of every row ([R] fp32), and the rows' norm
     ([R, 2] fp32: maximum, log-sum) that log_prob_grad takes.  margin: CUDA
     [R, K] float32, float16 or bfloat16 (row stride allowed); label: int32
-    [R], rows whose label is not a class are skipped."""
+    [R], rows whose label is not a class are skipped.  Detached from autograd:
+    log_prob_grad is the backward pass."""
     import torch
     dev = margin.device
     if _elsewhere(dev):
@@ -588,7 +592,8 @@ def policy_loss(margin, label, old_log_prob, advantage, ref_log_prob=None, weigh
     log_prob, label the sampled class; old_log_prob, advantage, ref_log_prob
     (None: no KL term) and weight (None: 1) [R] fp32; clip (low, high).  grad:
     True, a tensor to write to (the margins themselves included), or False for
-    the forward pass alone; hess: the diagonal curvature too."""
+    the forward pass alone; hess: the diagonal curvature too.  Detached from
+    autograd: margin.backward(result.grad) hands the gradient on."""
     import torch
     dev = margin.device
     if _elsewhere(dev):
@@ -629,7 +634,8 @@ def preference_loss(score, ref_score=None, item_begin=None, weight=None, beta: f
     """Preference loss over consecutive items (dp_preference_loss): item 2p is
     preferred to item 2p + 1.  score, ref_score: [R] fp32 CUDA; item_begin:
     int64 [2P + 1] offsets into the rows (None: every row is an item); weight:
-    [P] fp32."""
+    [P] fp32.  Detached from autograd: score.backward(result.grad) hands the
+    gradient on."""
     import torch
     dev = score.device
     if _elsewhere(dev):

@@ -188,3 +188,20 @@ def test_very_long_items_among_short_ones(dp, pairs, short, use_ref):
     off = 16 * e + 4 * e * np.repeat(np.abs(x).repeat(2), lengths)
     assert np.all(np.abs(r.grad.double().cpu().numpy() - q) <= beta * off)
     assert np.all(np.abs(r.hess.double().cpu().numpy() - h) <= beta * beta * off + 1e-22)
+
+
+def test_gradients_go_on_into_autograd_by_hand(dp):
+    """Results are detached; a gradient handed to backward() reaches what the margins came from."""
+    x = torch.randn(50, 8, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    w = torch.zeros(8, 5, device="cuda", requires_grad=True)
+    y = torch.arange(50, device="cuda", dtype=torch.int32) % 5
+    z = x @ w
+    logp, norm = dp.log_prob(z, y)
+    grad, _ = dp.log_prob_grad(z, y, norm, torch.ones(50, device="cuda"))
+    assert not logp.requires_grad and not grad.requires_grad
+    z.backward(grad)
+    p = torch.full((50, 5), 0.2, device="cuda")
+    hit = torch.nn.functional.one_hot(y.long(), 5).float()
+    assert (w.grad - x.T @ (hit - p)).abs().max() < 1e-4  # (fp32 sums of 50 terms of size 3)
+    with pytest.raises(dp.DPError, match="grad must be a tensor"):
+        dp.log_prob_grad(z, y, norm, torch.ones(50, device="cuda"), grad=False)
