@@ -976,9 +976,10 @@ template <class T, TileMode kMode, int KT, int NT, bool kExact>
 void launch_tile_of(const TileArgs& t, cudaStream_t s) {
   const u64 K = t.row.m.classes, size = (NT * K * sizeof(T) + 15) / 16 * 16 + (t.row.out.hess ? NT * K * 4 : 0);
   const u32 spread = bank_spread(row_words<T>(u32(K)));
-  constexpr bool kMayTurn = kExact ? bank_spread(row_words<T>(KT)) <= kTurnSpread : true;
+  // (of the up to eight classes that end at KT none but KT itself can meet so often)
+  constexpr bool kMayTurn = bank_spread(row_words<T>(KT)) <= kTurnSpread;
   auto* kernel = k_row_tile<T, kMode, KT, NT, kExact, kExact && kMayTurn>;
-  if constexpr (!kExact)
+  if constexpr (!kExact && kMayTurn)
     if (spread <= kTurnSpread) kernel = k_row_tile<T, kMode, KT, NT, kExact, true>;
   constexpr int kMost = NT * KT * (int(sizeof(T)) + 4) + 16;  // (one value for every call: other threads launch too)
   if constexpr (kMost > 48 * 1024)
@@ -1014,7 +1015,7 @@ void launch_tile(const TileArgs& t, cudaStream_t s) {
     if (K == 8) k_row_thread<T, kMode, 8><<<grid, 256, 0, s>>>(t);
     if (K == 16) k_row_thread<T, kMode, 16><<<grid, 256, 0, s>>>(t);
   } else if (K <= 16) {
-    launch_tile_exact<T, kMode, 1>(t, s);
+    launch_tile_exact<T, kMode, (sizeof(T) == 4 ? 2 : 1)>(t, s);  // (one fp32 class is always on its boundaries)
   } else if (K <= 20) {
     launch_tile_of<T, kMode, 20, 128, false>(t, s);
   } else if (K <= 24) {
@@ -1049,12 +1050,14 @@ bool use_tile(const Margins& m) {
 template <class T, bool kPolicy, int G>
 void launch_lanes(const RowArgs& a, u32 nvec, cudaStream_t s) {
   const u32 grid = grid_of((a.m.rows + 256 / G - 1) / (256 / G)), per_lane = (nvec + G - 1) / G;
-  if constexpr (G == 2 || G == 32) {
+  // (fp32 rows for two lanes have nine vectors at least, shorter ones a thread)
+  constexpr bool kShort = G == 32 || (G == 2 && sizeof(T) == 2);
+  if constexpr (kShort) {
     if (per_lane <= 2) k_row_loss<T, kPolicy, G, 2><<<grid, 256, 0, s>>>(a);
     else if (per_lane <= 3) k_row_loss<T, kPolicy, G, 3><<<grid, 256, 0, s>>>(a);
     else if (per_lane <= 4) k_row_loss<T, kPolicy, G, 4><<<grid, 256, 0, s>>>(a);
   }
-  if ((G != 2 && G != 32) || per_lane > 4) {
+  if (!kShort || per_lane > 4) {
     if (per_lane <= 5) k_row_loss<T, kPolicy, G, 5><<<grid, 256, 0, s>>>(a);
     else if (per_lane <= 6) k_row_loss<T, kPolicy, G, 6><<<grid, 256, 0, s>>>(a);
     else k_row_loss<T, kPolicy, G, 8><<<grid, 256, 0, s>>>(a);
@@ -1187,8 +1190,8 @@ void launch_grad_of(const GradArgs& a, cudaStream_t s) {
     row.label = a.label;
     row.out = a.out;
     launch_tile<T, kTileGrad>(TileArgs{row, a.norm, a.weight}, s);
-  } else if (nvec <= 8) {
-    launch_grad_pieces<T, 2>(a, nvec, s);
+  } else if (sizeof(T) == 2 && nvec <= 8) {  // (fp32 rows this short take a thread)
+    if constexpr (sizeof(T) == 2) launch_grad_pieces<T, 2>(a, nvec, s);
   } else if (nvec <= 16) {
     launch_grad_pieces<T, 4>(a, nvec, s);
   } else if (nvec <= 32) {
