@@ -205,3 +205,58 @@ def test_gradients_go_on_into_autograd_by_hand(dp):
     assert (w.grad - x.T @ (hit - p)).abs().max() < 1e-4  # (fp32 sums of 50 terms of size 3)
     with pytest.raises(dp.DPError, match="grad must be a tensor"):
         dp.log_prob_grad(z, y, norm, torch.ones(50, device="cuda"), grad=False)
+
+
+PIECE = 8192  # rows that a block of the whole-device form takes
+LONG = 1 << 18
+
+
+@pytest.mark.parametrize("use_ref,smoothing", [(False, 0.0), (True, 0.1)])
+@pytest.mark.parametrize("begin,tail", [
+    ([0, 8191, 300_000], 0), ([8192, 5 * 8192, 40 * 8192], 5), ([8193, 8192 * 17 + 1, 8192 * 38 - 1], 1),
+    ([8191, 8191, 8191 + LONG], 0), ([3, 3 + LONG, 3 + LONG], 9),
+    # pairs just below, at and past the length that is cut into pieces, and one that makes their average long
+    ([100, 9000, 32_867, 32_867, 65_635, 70_000, 98_404, 500_000, 1_200_000], 3),
+    # eight pairs, empty ones and single rows among them
+    (list(np.cumsum([16_384, 0, 0, 1, 0, 1_000_003, 3, 8192, 24_576, 250_001, 16_385, 1, 0, 400_000, 400_001, 7, 2])), 0)])
+def test_few_pairs_of_very_many_rows_lose_no_piece(dp, begin, tail, use_ref, smoothing):
+    """Small integers whose sums are exact in any order: a piece that is left out, or
+    counted twice, moves its pair's loss by twenty times the bound or more."""
+    begin = np.array(begin)
+    pairs, rows = len(begin) // 2, int(begin[-1]) + tail
+    assert pairs <= 8 and rows // pairs >= LONG
+    rng = np.random.default_rng(rows)
+    gap = rng.integers(-2, 3, rows).astype(np.float32)
+    cuts = np.union1d(np.arange(0, rows, PIECE), begin[begin < rows])
+    empty = np.add.reduceat(gap, cuts) == 0  # (no piece of an item sums to nothing)
+    gap[cuts[empty]] += 1
+    pieces = np.add.reduceat(gap, cuts)
+    assert np.all(pieces != 0)
+    refs = rng.integers(-9, 10, rows).astype(np.float32) if use_ref else None
+    score = gap + refs if use_ref else gap
+    run = np.concatenate([[0.0], np.cumsum(gap.astype(np.float64))])
+    total = run[begin[1:]] - run[begin[:-1]]
+    beta, smooth = 2.0 ** -10, float(np.float32(smoothing))
+    x = beta * (total[0::2] - total[1::2])
+    w = (0.5 + rng.random(pairs)).astype(np.float32)
+    if pairs > 4:
+        w[4] = 0.0
+    up = lambda v: None if v is None else torch.from_numpy(v).cuda()  # noqa: E731
+    r = dp.preference_loss(up(score), ref_score=up(refs), item_begin=up(begin), weight=up(w), beta=beta,
+                           smoothing=smooth, hess=True)
+    e = 2.0 ** -24
+    up_, down = 1 / (1 + np.exp(-x)), 1 / (1 + np.exp(x))
+    loss = (1 - smooth) * np.logaddexp(0, -x) + smooth * np.logaddexp(0, x)
+    slope, bend = smooth * up_ - (1 - smooth) * down, up_ * down
+    # a dozen roundings of terms no larger than 1 + |x|
+    bound = 16 * e * (1 + np.abs(x))
+    # what a piece of the smallest sum moves a loss by at least
+    assert beta * np.abs(pieces).min() * np.minimum(up_, down).min() * (1 - 2 * smooth) > 20 * bound.max()
+    assert np.all(np.abs(r.loss.double().cpu().numpy() - w * loss) <= w * bound)
+    lengths = np.diff(begin)
+    rowwise = lambda a, b, out: np.concatenate([np.full(begin[0], out), np.repeat(np.stack([a, b], 1).reshape(-1), lengths),  # noqa: E731
+                                                np.full(tail, out)])
+    g, h = r.grad.double().cpu().numpy(), r.hess.double().cpu().numpy()
+    assert np.all(np.abs(g - rowwise(w * beta * slope, -w * beta * slope, 0.0)) <= rowwise(beta * bound, beta * bound, 0.0))
+    want = np.maximum(w * beta * beta * bend, 1e-16)
+    assert np.all(np.abs(h - rowwise(want, want, 1e-16)) <= rowwise(beta * beta * bound, beta * beta * bound, 0.0) + 1e-22)
