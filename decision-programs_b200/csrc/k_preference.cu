@@ -34,7 +34,7 @@ __device__ __forceinline__ PairResult pair_result(const PairLoss& a, float diffe
 
 // ---- consecutive items ------------------------------------------------------
 // Every row an item: a thread takes pairs of rows side by side.  Bound by memory:
-// 2M rows in 1M pairs, gradient and curvature, 5.3 us (32 MB, part of it from L2).
+// 2M rows in 1M pairs, gradient and curvature, 5.5 us (28 MB, part of it from L2).
 template <bool kWide>
 __global__ void __launch_bounds__(256) k_preference_rows(PairLoss a, u64 rows, u64 pairs) {
   const u64 step = u64(gridDim.x) * blockDim.x, first = u64(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -418,8 +418,9 @@ __global__ void __launch_bounds__(512) k_preference_spread(PairLoss a, u64 rows,
 // Three launches: every pair's terms once, in the pairs' order (two gathers of
 // scores a pair); then the terms summed by row over the list of (row, pair)
 // that the plan holds sorted by row, a warp taking kPairChunk entries whatever
-// rows they belong to, so that one row in very many pairs costs no more than
-// many rows in few; then the rows that reach over several chunks.  Bound by
+// rows they belong to; then the rows that reach over several chunks, a warp
+// each, which is what rows in very many pairs cost (8M pairs that share one row:
+// 589 us, of strongly skewed rows 207).  Bound by
 // the gathers, two of 4-byte scores and two of 8-byte terms a pair, a random
 // sector a lane, of which L1 takes 0.7 to 0.8 a clock and SM: 8M pairs over 1M
 // rows 170 us (82 + 83 + 5).  One thread a row, evaluating each pair from both
@@ -589,7 +590,8 @@ __global__ void __launch_bounds__(256) k_pair_joins(PairLoss a, const PairEntry*
 }
 
 // ---- the plan: (row, pair) entries sorted by row, by a least-significant-
-// digit radix sort, which keeps the pairs of a row in their order.
+// digit radix sort, which keeps the pairs of a row in their order.  8M pairs
+// over 1M rows take 0.9 to 1.2 ms, as long as five to seven runs.
 __global__ void __launch_bounds__(256) k_pair_entries(const int2* __restrict__ pair, u64 pairs, u64 rows, PairEntry* out,
                                                       unsigned long long* bad) {
   for (u64 p = u64(blockIdx.x) * blockDim.x + threadIdx.x; p < pairs; p += u64(gridDim.x) * blockDim.x) {

@@ -416,7 +416,9 @@ __device__ __forceinline__ void skip_row(const RowArgs& a, u64 r, bool writer) {
   else a.norm[r] = make_float2(0.f, 0.f);
 }
 
-// G lanes of a warp a row, V vectors a lane, kept in registers: one read, no
+// G lanes of a warp a row, V vectors a lane, kept in registers (with eight, the
+// policy loss has 56 to 84 bytes a thread of a 16-bit row in local memory, of an
+// fp32 row 4 to 20: four blocks an SM leave 64 registers): one read, no
 // barrier, and enough warps for memory to stay busy.  134M fp32 margins in rows
 // of 1000: forward and backward 157 us, 6.9 TB/s (bound by DRAM); bf16 in rows
 // of 2048: 95 us, 5.7 TB/s (DRAM and the exponential unit).
@@ -841,7 +843,7 @@ constexpr u32 kTurnSpread = 4;
 
 // NT rows a block; KT: the row length (kExact) or the most that it may be.  fp32
 // rows are bound by DRAM (6.7M x 10, forward and backward: 107 us, 6.5 TB/s),
-// 16-bit ones by instructions (the same in bf16: 92 us, 3.8 TB/s).
+// 16-bit ones by instructions (the same in bf16: 93 us, 4.6 TB/s).
 template <class T, TileMode kMode, int KT, int NT, bool kExact, bool kTurn>
 __global__ void __launch_bounds__(NT) k_row_tile(TileArgs t, u32 spread_given) {
   extern __shared__ uint4 tile16[];
@@ -1039,7 +1041,7 @@ void launch_tile(const TileArgs& t, cudaStream_t s) {
 // and lanes: 36 fp32 classes 101 and 117 us forward and backward, 40 104 and
 // 96; 24 bf16 classes 86 and 105, 32 103 and 82); up to 64 where rows lie off
 // the 16-byte boundaries, which lanes would take element by element at both
-// ends (33 bf16 classes 79 and 145 us, fp32 92 and 150).
+// ends (33 bf16 classes 84 and 145 us, fp32 98 and 150).
 template <class T>
 bool use_tile(const Margins& m) {
   const bool even = m.classes * sizeof(T) % 16 == 0 && on_boundaries(m.z, m.rows, m.stride, sizeof(T), 16);
